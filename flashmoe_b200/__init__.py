@@ -13,12 +13,12 @@ import ctypes as C
 import os
 
 from . import _native as N
-from . import cb, reference, router
+from . import cb, fp8, reference, router
 from .cb import get_local_rank
 from .jit import (ActivationType, ContextHandle, DataType, ForwardArgs, InitArgs, MLPType,
                   Topology, _get_compiled, specialised_library)
 
-__all__ = ["initialize", "forward", "finalize", "get_workspace_bytes", "router", "reference", "cb", "get_local_rank", "InitArgs",
+__all__ = ["initialize", "forward", "finalize", "get_workspace_bytes", "router", "fp8", "reference", "cb", "get_local_rank", "InitArgs",
            "ForwardArgs", "ContextHandle", "Topology", "MLPType", "ActivationType", "DataType",
            "FlashMoEError"]
 FlashMoEError = N.FlashMoEError

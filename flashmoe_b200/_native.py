@@ -14,7 +14,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 SRC_DIR = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "lib" / "libflashmoe_b200.so"
-SOURCES = ("router.cu", "moe_kernel.cu", "abi.cu")
+SOURCES = ("router.cu", "moe_kernel.cu", "abi.cu", "select.cu", "fp8_quantize.cu", "fp8_matmul.cu", "fp8_experts.cu")
 NVCC_FLAGS = ("-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
               "-Xcompiler", "-fPIC", "-shared", "-ldl")
 
@@ -60,6 +60,41 @@ class Geometry(C.Structure):
                                                                   ("reserved", C.c_int32)]
 
 
+def _fields(pointers: str, ints: str, **after):
+    """Pointer fields, then int32 fields; `after` puts fields of other types behind a named one."""
+    out = []
+    for n in pointers.split():
+        out += [(n, C.c_void_p)] + after.get(n, [])
+    for n in ints.split():
+        out += [(n, C.c_int32)] + after.get(n, [])
+    return out
+
+
+class SelectArgsC(C.Structure):
+    _fields_ = _fields("logits bias ids weights expert_counts offsets positions",
+                       "num_tokens num_experts top_k data_type score num_groups top_groups group_score renormalize",
+                       renormalize=[("scale", C.c_float), ("device_id", C.c_int32)])
+
+
+class Fp8QuantizeArgsC(C.Structure):
+    _fields_ = _fields("x q scale positions", "copies rows cols num_matrices block_rows data_type device_id")
+
+
+class Fp8MatmulArgsC(C.Structure):
+    _fields_ = _fields("a a_scale w w_scale out offsets", "m n k num_experts data_type device_id")
+
+
+class Fp8GatedArgsC(C.Structure):
+    _fields_ = _fields("a a_scale up up_scale up_v up_v_scale q scale offsets",
+                       "m ffn_size k num_experts act_type device_id")
+
+
+class Fp8ExpertsArgsC(C.Structure):
+    _fields_ = _fields("tokens offsets positions weights up up_scale up_v up_v_scale down down_scale out workspace",
+                       "num_tokens token_dim ffn_size num_experts top_k data_type act_type device_id",
+                       workspace=[("workspace_bytes", C.c_int64)])
+
+
 # name -> (restype, argtypes); the single source of truth for the symbol-export test too
 SIGNATURES = {
     "fmoe_ctx_create": (C.c_int, [C.POINTER(ModelDesc), C.POINTER(EpDesc), C.c_void_p,
@@ -86,6 +121,13 @@ SIGNATURES = {
     "fmoe_router_destroy": (C.c_int, [C.c_void_p, C.c_void_p]),
     "fmoe_router_forward_static": (C.c_int, [C.POINTER(ModelDesc), C.c_int32, C.POINTER(RouterArgsC),
                                             C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
+    "fmoe_router_select": (C.c_int, [C.c_void_p, C.POINTER(SelectArgsC), C.c_void_p]),
+    "fmoe_fp8_quantize": (C.c_int, [C.POINTER(Fp8QuantizeArgsC), C.c_void_p]),
+    "fmoe_fp8_matmul": (C.c_int, [C.POINTER(Fp8MatmulArgsC), C.c_void_p]),
+    "fmoe_fp8_gated_matmul": (C.c_int, [C.POINTER(Fp8GatedArgsC), C.c_void_p]),
+    "fmoe_fp8_workspace_bytes": (C.c_int, [C.POINTER(Fp8ExpertsArgsC), C.POINTER(C.c_int64)]),
+    "fmoe_fp8_experts": (C.c_int, [C.POINTER(Fp8ExpertsArgsC), C.c_void_p]),
+    "fmoe_fp8_last_status": (C.c_int, [C.c_int32, C.c_void_p, C.POINTER(Status)]),
     "fmoe_forward_host": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                     C.POINTER(RouterArgsC), C.POINTER(ForwardArgsC), C.c_void_p]),
     "fmoe_forward_host_async": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,

@@ -91,6 +91,22 @@ int make_map(CUtensorMap* out, int ab_format, const void* base, uint64_t rows, u
 }
 
 }  // namespace
+
+int make_byte_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return set_error(FMOE_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {cols};
+  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(FMOE_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
+  return FMOE_OK;
+}
+
 }  // namespace fmoe
 
 using namespace fmoe;
@@ -149,6 +165,21 @@ struct fmoe_router {
 };
 
 namespace fmoe {
+
+int routing_targets(fmoe_ctx* moe, int S, int E, int k, int device, TokenSlot** table, Route** routes, int* capacity,
+                    int* round_ec) {
+  if (moe->poisoned)
+    return set_error(FMOE_ERR_DEVICE_TIMEOUT, "an earlier forward of this context ran out of a device-side wait "
+                                              "(see fmoe_last_status); destroy the context and create a new one");
+  const fmoe_model_desc& m = moe->model;
+  if (m.tokens_per_rank != S || m.num_experts != E || m.top_k != k || moe->device != device)
+    return set_error(FMOE_ERR_INVALID_ARG, "the MoE context has other tokens, experts, top_k or another device");
+  *table = const_cast<TokenSlot*>(moe->params.table);
+  *routes = const_cast<Route*>(moe->params.routes);
+  *capacity = m.expert_peer_capacity;
+  *round_ec = moe->geo.round_ec;
+  return FMOE_OK;
+}
 
 int validate_model(const fmoe_model_desc* m) {
   if (m == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "model description is null");

@@ -133,5 +133,11 @@ extern unsigned long long g_launches;
 // host-side helpers shared by the translation units that export C entry points
 int set_error(int code, const std::string& msg);   // records the thread's last error text
 int validate_model(const fmoe_model_desc* m);
+// TMA descriptor of a row-major byte matrix [rows, cols]: boxes of box_rows x 128 bytes, 128-byte
+// swizzle, zeros outside; base 16-byte aligned, cols a multiple of 16
+int make_byte_map(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows);
+// Where a context's forward looks for its routing (checked against S, E, k and the device)
+int routing_targets(fmoe_ctx* moe, int S, int E, int k, int device, TokenSlot** table, Route** routes, int* capacity,
+                    int* round_ec);
 
 }  // namespace fmoe

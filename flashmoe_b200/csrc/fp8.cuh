@@ -1,0 +1,165 @@
+// What the 8-bit kernels share: the block format, tensor-core and conversion wrappers, launch helpers.
+//
+// A matrix in 8 bits is a row-major array of e4m3 codes and one fp32 scale per block: 1 x 128 values
+// of a row for activations (scale [rows, ceil(cols / 128)]), 128 x 128 values for weights (scale
+// [matrices, ceil(rows / 128), ceil(cols / 128)]).  A code stands for (its value) * (its block's scale).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace fmoe::fp8 {
+
+constexpr int kBlock = 128;          // values per scale along a row, rows per scale of a weight block
+constexpr float kE4m3Max = 448.0f;   // largest finite e4m3 value
+
+__host__ __device__ constexpr int blocks_of(int n) { return (n + kBlock - 1) / kBlock; }
+
+// ---- quantisation arithmetic ----------------------------------------------------------------
+// scale = amax / 448, code = e4m3(448 x / amax), all in IEEE fp32.  For 16-bit x the product 448 x
+// is exact and the quotient correctly rounded, so the code is the one infinite precision would give:
+// a quotient of two such numbers that is not a midpoint of two codes is at least 2^-11 of itself away
+// from one, far more than half an fp32 step.
+// Very large blocks are scaled down by a power of two first (448 x must stay finite); values that
+// underflow by it are below 2^-200 of amax and have the code 0 either way.
+struct Quantizer {
+  float num, den;   // code = e4m3((num x) / den)
+  __device__ __forceinline__ explicit Quantizer(float amax) {
+    const float pre = amax > 0x1p+100f ? 0x1p-20f : 1.0f;
+    num = kE4m3Max * pre;
+    den = amax > 0.0f ? amax * pre : (amax == 0.0f ? 1.0f : amax);   // an empty block: codes 0; NaN stays
+  }
+  __device__ __forceinline__ float scaled(float x) const { return __fdiv_rn(__fmul_rn(x, num), den); }
+};
+__device__ __forceinline__ float block_scale(float amax) { return __fdiv_rn(amax, kE4m3Max); }
+// Two values to two codes (lo in the low byte), round to nearest even.
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+  return to_e4m3x2(a, b) | (to_e4m3x2(c, d) << 16);
+}
+// |x| as an integer that orders like the value, with NaN above infinity: a maximum over these keeps
+// a NaN, which fmaxf would drop.
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// ---- element types ----------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// 16 bytes as 16 / sizeof(T) floats
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& u, float (&f)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      f[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float (&f)[16 / sizeof(T)]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(f[i]);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ float activate(float x, int act) {
+  switch (act) {
+    case FMOE_ACT_SILU: return x / (1.0f + expf(-x));
+    case FMOE_ACT_GELU: return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+    case FMOE_ACT_RELU: return fmaxf(x, 0.0f);
+    default: return x;
+  }
+}
+
+// ---- tensor core -------------------------------------------------------------------------------
+// Instruction descriptor for kind::f8f6f4: fp32 accumulate (bit 4), A and B e4m3 (format 0), both
+// K-major, N >> 3 at [17,23), M >> 4 at [24,29).
+__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+// D[tmem] (+)= A[smem] * B[smem]^T over 32 bytes of K, issued by one thread.
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Two independent fp32 multiply-adds.
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+
+// ---- host side -----------------------------------------------------------------------------------
+// Makes `device` current for the scope and puts the caller's device back.
+struct OnDevice {
+  int prev = -1;
+  cudaError_t err;
+  explicit OnDevice(int device) {
+    int cur = -1;
+    err = cudaGetDevice(&cur);
+    if (err == cudaSuccess && cur != device) {
+      err = cudaSetDevice(device);
+      if (err == cudaSuccess) prev = cur;
+    }
+  }
+  ~OnDevice() { if (prev >= 0) cudaSetDevice(prev); }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+};
+inline bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+inline int element_bytes(int data_type) { return data_type == FMOE_DT_FP32 ? 4 : 2; }
+int sm_count(int device);   // cached per device
+
+}  // namespace fmoe::fp8

@@ -1,0 +1,543 @@
+// Products of 8-bit matrices with block scales on the tensor cores, dense and by expert:
+//
+//   out[r, f] = sum over 128-blocks b of k:  sa[r, b] * sw[f / 128, b] * (sum over i in b of a[r, i] w[f, i])
+//
+// The inner sums are tcgen05 products of e4m3 (exact products, fp32 accumulation in TMEM), one
+// TMEM accumulator per block of k; the outer sum is taken by the epilogue warps, which read each
+// block's accumulator, scale it and add it to fp32 registers.  The tensor core never sees a scale, so
+// any fp32 scales work, and no sum crosses a block boundary unscaled.
+//
+// One persistent CTA per SM: warp 0 loads tiles (TMA), warp 1 issues the MMAs, warps 2..9 scale and
+// add.  A tile is 128 rows x 256 features (the gated form: 128 features of up and the same 128 of
+// up_v); the two TMEM accumulators of 256 columns let the MMAs of one block run while the other
+// block's sums are read.
+#include <atomic>
+#include <cstdlib>
+#include <mutex>
+#include <type_traits>
+
+#include "fp8.cuh"
+
+namespace fmoe::fp8 {
+namespace {
+
+using namespace fmoe::ptx;
+
+constexpr int kThreads = 320;                  // TMA warp, MMA warp, eight epilogue warps
+constexpr int kEpilogueWarps = 8;
+constexpr int kMaxExperts = 1024;
+constexpr uint32_t kBoxBytes = 128 * kBlock;   // 128 rows of one k block: 16 KB
+constexpr int kStages = 4;
+constexpr uint32_t kStageBytes = 3 * kBoxBytes;
+
+struct Codes {};   // "output type" of the gated form
+
+__device__ fmoe_status g_status;   // first wait that ran out (fmoe_fp8_last_status)
+
+struct ProductParams {
+  int m, n, k;
+  int kblocks, nblocks;        // 128-blocks along k and n
+  int experts, tiles_n;
+  const int32_t* offsets;      // null: one product over all m rows
+  const float* a_scale;
+  const float* w_scale[2];     // the gated form: up, up_v
+  void* out;                   // rows, or the codes of the gated form
+  float* out_scale;            // gated form
+  int act, has_v;              // gated form
+  int wide;                    // output rows may be stored 32 bytes at a time
+  long long spin_limit;
+};
+
+struct Tile {
+  int expert, row0, row_end, n0;
+};
+
+// Which rows each expert has and how many tiles come before it; filled once per CTA.
+struct TileTable {
+  int begin[kMaxExperts];
+  int rows[kMaxExperts];
+  int first[kMaxExperts + 1];
+};
+
+__device__ __forceinline__ bool find_tile(const TileTable& t, int experts, int tile, int tile_m, int tile_n, Tile& out) {
+  if (tile >= t.first[experts]) return false;
+  int lo = 0, hi = experts - 1;
+  while (lo < hi) {                      // the last expert that begins at or before this tile
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= tile) lo = mid; else hi = mid - 1;
+  }
+  const int m_tiles = (t.rows[lo] + tile_m - 1) / tile_m, i = tile - t.first[lo];
+  out.expert = lo;                       // rows first: neighbouring CTAs share a weight tile
+  out.row0 = t.begin[lo] + (i % m_tiles) * tile_m;
+  out.row_end = t.begin[lo] + t.rows[lo];
+  out.n0 = (i / m_tiles) * tile_n;
+  return true;
+}
+
+// Called by every thread; `experts` entries, tile counts summed by warp 0.
+__device__ void fill_table(TileTable& t, const ProductParams& p, int tile_m) {
+  for (int e = threadIdx.x; e < p.experts; e += blockDim.x) {
+    int begin = 0, end = p.m;
+    if (p.offsets != nullptr) {          // whatever the array holds, rows stay inside [0, m)
+      begin = min(max(__ldg(p.offsets + e), 0), p.m);
+      end = min(max(__ldg(p.offsets + e + 1), begin), p.m);
+    }
+    t.begin[e] = begin;
+    t.rows[e] = end - begin;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int before = 0;
+    for (int e0 = 0; e0 < p.experts; e0 += 32) {
+      const int e = e0 + threadIdx.x;
+      const int own = e < p.experts ? ((t.rows[e] + tile_m - 1) / tile_m) * p.tiles_n : 0;
+      int sum = own;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, d);
+        if (static_cast<int>(threadIdx.x) >= d) sum += v;
+      }
+      if (e < p.experts) t.first[e] = before + sum - own;
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (threadIdx.x == 0) t.first[p.experts] = before;
+  }
+  __syncthreads();
+}
+
+__device__ __noinline__ void wait_failed(volatile uint32_t* abort_word, int phase, int detail) {
+  if (atomicCAS(&g_status.code, FMOE_OK, FMOE_ERR_DEVICE_TIMEOUT) == FMOE_OK) {
+    g_status.phase = phase;
+    g_status.rank = 0;
+    g_status.cta = blockIdx.x;
+    g_status.detail = detail;
+  }
+  *abort_word = 1;
+}
+
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Waits for this thread's TMEM loads; naming the registers keeps their uses behind the wait.
+__device__ __forceinline__ void tmem_wait_16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// 128 features of one row, in order in acc[64] (pairs), to dst; `valid` of them exist.
+template <typename Out>
+__device__ __forceinline__ void store_features(Out* dst, const uint64_t (&acc)[64], int valid, bool wide) {
+  constexpr int kPer = 32 / sizeof(Out);
+#pragma unroll
+  for (int g = 0; g < 128 / kPer; ++g) {
+    float f[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) {
+      const float2 v = unpack2(acc[g * (kPer / 2) + i]);
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    }
+    if (wide && (g + 1) * kPer <= valid) {
+      uint32_t w[8];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float h[kPer / 2];
+#pragma unroll
+        for (int i = 0; i < kPer / 2; ++i) h[i] = f[q * (kPer / 2) + i];
+        const uint4 u = pack16<Out>(h);
+        w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
+      }
+      st_global_32(dst + g * kPer, w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (g * kPer + i < valid) dst[g * kPer + i] = from_float<Out>(f[i]);
+    }
+  }
+}
+
+struct SharedTail {
+  uint64_t full[kStages], empty[kStages];
+  uint64_t acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  uint32_t abort_word;
+  uint32_t amax[2][2][128];   // [tile parity][column half][row]
+  uint64_t amax_full[4];      // both halves' maxima of a quarter's rows are in
+  TileTable table;
+};
+
+// Rows on the TMEM lanes, features on its columns.
+template <typename Out>
+__global__ void __launch_bounds__(kThreads, 1)
+product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w0,
+               const __grid_constant__ CUtensorMap map_w1, const ProductParams p) {
+  constexpr bool kGated = std::is_same_v<Out, Codes>;
+  constexpr int kTileM = 128, kTileN = kGated ? 128 : 256;
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  unsigned char* ring = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);   // swizzle atoms are 1024 bytes
+  SharedTail& sh = *reinterpret_cast<SharedTail*>(ring + kStages * kStageBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WaitCtx wc{&sh.abort_word, p.spin_limit};
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&sh.acc_full[i], 1); mbar_init(&sh.acc_empty[i], kEpilogueWarps); }
+    for (int i = 0; i < 4; ++i) mbar_init(&sh.amax_full[i], 2);
+    sh.abort_word = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sh.tmem_base, 512);
+    tmem_relinquish();
+  }
+  fill_table(sh.table, p, kTileM);
+  tc_fence_after_sync();
+  const uint32_t tmem = sh.tmem_base;
+  const bool second = !kGated || p.has_v != 0;   // whether the second 128 weight rows exist
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t bytes = (second ? 3 : 2) * kBoxBytes;
+      int issued = 0;
+      Tile t;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += gridDim.x) {
+        const int w_row = t.expert * p.n + t.n0;   // (host: experts * n fits an int)
+        for (int kb = 0; kb < p.kblocks; ++kb, ++issued) {
+          const int s = issued % kStages;
+          if (!mbar_wait(&sh.empty[s], ((issued / kStages) & 1) ^ 1, wc)) {
+            wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_EMPTY, i);
+            ok = false;
+            break;
+          }
+          unsigned char* stage = ring + s * kStageBytes;
+          mbar_expect_tx(&sh.full[s], bytes);
+          tma_load_2d(stage, &map_a, &sh.full[s], kb * kBlock, t.row0);
+          tma_load_2d(stage + kBoxBytes, &map_w0, &sh.full[s], kb * kBlock, w_row);
+          if (second) tma_load_2d(stage + 2 * kBoxBytes, &map_w1, &sh.full[s], kb * kBlock, kGated ? w_row : w_row + 128);
+        }
+      }
+      // no copy may be in flight when the CTA leaves (all have been waited for unless a wait ran out)
+      const WaitCtx last{nullptr, p.spin_limit};
+      for (int j = max(0, issued - kStages); j < issued; ++j) mbar_wait(&sh.full[j % kStages], (j / kStages) & 1, last);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_e4m3(128, second ? 256 : 128);
+      int done = 0;
+      Tile t;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += gridDim.x) {
+        for (int kb = 0; kb < p.kblocks; ++kb, ++done) {
+          const int s = done % kStages, b = done & 1;
+          if (!mbar_wait(&sh.acc_empty[b], ((done >> 1) & 1) ^ 1, wc)) {
+            wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_EMPTY, i);
+            ok = false;
+            break;
+          }
+          if (!mbar_wait(&sh.full[s], (done / kStages) & 1, wc)) {
+            wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_FULL, i);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t stage = smem_u32(ring + s * kStageBytes);
+          const uint64_t da = umma_desc_sw128(stage), dw = umma_desc_sw128(stage + kBoxBytes);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)   // 32 bytes of k each
+            umma_f8(tmem + b * 256, da + 2 * q, dw + 2 * q, idesc, q != 0);
+          umma_commit(&sh.empty[s]);
+          umma_commit(&sh.acc_full[b]);
+        }
+      }
+      // no MMA may be running when TMEM is freed
+      const WaitCtx last{nullptr, p.spin_limit};
+      if (done > 0) mbar_wait(&sh.acc_full[(done - 1) & 1], ((done - 1) >> 1) & 1, last);
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;   // TMEM lanes of this warp; its half of the columns
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const int r = quarter * 32 + lane;
+    int done = 0, parity = 0;
+    Tile t;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += gridDim.x, parity ^= 1) {
+      const int row = t.row0 + r;
+      const bool live = row < t.row_end;
+      // scales of this thread's row, and of its first and last 64 columns; two blocks ahead in registers
+      const float* sa = live ? p.a_scale + static_cast<size_t>(row) * p.kblocks : nullptr;
+      const int nb = t.n0 / kBlock + (kGated ? 0 : half);
+      const size_t w_at = (static_cast<size_t>(t.expert) * p.nblocks + nb) * p.kblocks;
+      const float* sw0 = nb < p.nblocks ? p.w_scale[0] + w_at : nullptr;
+      const float* sw1 = kGated ? (second ? p.w_scale[1] + w_at : nullptr) : sw0;
+      auto scale_at = [&](const float* s, int kb) { return s != nullptr && kb < p.kblocks ? __ldg(s + kb) : 0.0f; };
+      float a0 = scale_at(sa, 0), a1 = scale_at(sa, 1);
+      float u0 = scale_at(sw0, 0), u1 = scale_at(sw0, 1);
+      float v0 = kGated ? scale_at(sw1, 0) : 0.0f, v1 = kGated ? scale_at(sw1, 1) : 0.0f;
+      uint64_t acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = 0;
+      for (int kb = 0; kb < p.kblocks; ++kb, ++done) {
+        const int b = done & 1;
+        const float a = a0, u = u0, v = v0;
+        a0 = a1; u0 = u1; v0 = v1;
+        a1 = scale_at(sa, kb + 2);
+        u1 = scale_at(sw0, kb + 2);
+        if constexpr (kGated) v1 = scale_at(sw1, kb + 2);
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[b], (done >> 1) & 1, wc));
+        if (!ok) {
+          if (lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_FULL, i);
+          break;
+        }
+        tc_fence_after_sync();
+        const uint64_t s0 = pack2(a * u, a * u), s1 = kGated ? pack2(a * v, a * v) : s0;
+        // columns of chunk c: this half's 128, or 64 of up and the same 64 of up_v
+        auto column = [&](int c) { return kGated ? (c < 4 ? half * 64 + c * 16 : 128 + half * 64 + (c - 4) * 16) : half * 128 + c * 16; };
+        uint32_t d[2][16];
+        tmem_ld_16(taddr + b * 256 + column(0), d[0]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          tmem_wait_16(d[c & 1]);
+          if (c < 7) {
+            tmem_ld_16(taddr + b * 256 + column(c + 1), d[(c + 1) & 1]);
+          } else {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.acc_empty[b]);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            acc[c * 8 + j] = fma2(pack2(d[c & 1][2 * j], d[c & 1][2 * j + 1]), c < 4 ? s0 : s1, acc[c * 8 + j]);
+        }
+      }
+      if (!ok) break;
+      if constexpr (kGated) {
+        // h = act(up) * up_v of 64 features of this row; the block's maximum with the other half's warp
+        const int col = t.n0 + half * 64;
+        uint32_t amax = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float2 g = unpack2(acc[j]), w = unpack2(acc[32 + j]);
+          float h0 = activate(g.x, p.act), h1 = activate(g.y, p.act);
+          if (second) { h0 *= w.x; h1 *= w.y; }
+          if (col + 2 * j >= p.n) h0 = h1 = 0.0f;   // (n is even)
+          amax = max(amax, max(abs_bits(h0), abs_bits(h1)));
+          acc[j] = pack2(h0, h1);
+        }
+        sh.amax[parity][half][r] = amax;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.amax_full[quarter]);
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.amax_full[quarter], parity, wc));
+        if (!ok) {
+          if (lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TASK, i);
+          break;
+        }
+        const float top = __uint_as_float(max(sh.amax[parity][0][r], sh.amax[parity][1][r]));
+        if (live) {
+          const Quantizer z(top);
+          unsigned char* q = static_cast<unsigned char*>(p.out) + static_cast<size_t>(row) * p.n + col;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            if (col + g * 16 < p.n) {   // (n is a multiple of 16)
+              uint32_t w[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float2 lo = unpack2(acc[g * 8 + 2 * x]), hi = unpack2(acc[g * 8 + 2 * x + 1]);
+                w[x] = to_e4m3x4(z.scaled(lo.x), z.scaled(lo.y), z.scaled(hi.x), z.scaled(hi.y));
+              }
+              *reinterpret_cast<uint4*>(q + g * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          if (half == 0) p.out_scale[static_cast<size_t>(row) * p.nblocks + t.n0 / kBlock] = block_scale(top);
+        }
+      } else {
+        const int col = t.n0 + half * 128;
+        if (live && col < p.n)
+          store_features<Out>(static_cast<Out*>(p.out) + static_cast<size_t>(row) * p.n + col, acc, p.n - col, p.wide != 0);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+constexpr size_t kProductSmem = 1024 + kStages * kStageBytes + sizeof(SharedTail);
+static_assert(kProductSmem <= 227 * 1024, "shared memory of one CTA");
+
+// What a launch needs to know about a device, looked up once.
+struct DeviceFacts {
+  int sms = 0;
+  long long spin_limit = 0;
+};
+constexpr int kMaxDevices = 64;
+const DeviceFacts& facts(int device) {
+  static DeviceFacts all[kMaxDevices];
+  static std::once_flag once[kMaxDevices];
+  std::call_once(once[device], [&] {
+    if (cudaDeviceGetAttribute(&all[device].sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) all[device].sms = 148;
+    const char* ms = std::getenv("FMOE_SPIN_LIMIT_MS");
+    all[device].spin_limit = spin_limit_cycles(ms ? std::atof(ms) : 2000.0, device);
+  });
+  return all[device];
+}
+
+template <typename Out>
+int launch_product_of(const ProductParams& p, const CUtensorMap (&maps)[3], int grid, int device, cudaStream_t stream) {
+  static std::atomic<unsigned long long> prepared{0};   // devices whose shared-memory limit was raised
+  if (!(prepared.load(std::memory_order_acquire) >> device & 1)) {
+    const cudaError_t e = cudaFuncSetAttribute(product_kernel<Out>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(kProductSmem));
+    if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("8-bit product: ") + cudaGetErrorString(e));
+    prepared.fetch_or(1ull << device, std::memory_order_release);
+  }
+  product_kernel<Out><<<grid, kThreads, kProductSmem, stream>>>(maps[0], maps[1], maps[2], p);
+  ++g_launches;
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("8-bit product launch: ") + cudaGetErrorString(e));
+  return FMOE_OK;
+}
+
+// The checks that both products share.
+int check_product(const void* a, const float* a_scale, const void* w, const float* w_scale, const int32_t* offsets, int m,
+                  int n, int k, int experts, int device) {
+  if (m < 0 || n < 1 || k < 1) return set_error(FMOE_ERR_INVALID_ARG, "m must not be negative, n and k must be positive");
+  if (experts < 1 || experts > kMaxExperts)
+    return set_error(FMOE_ERR_INVALID_ARG, "num_experts must be between 1 and " + std::to_string(kMaxExperts));
+  if (device < 0 || device >= kMaxDevices) return set_error(FMOE_ERR_INVALID_ARG, "device_id out of range");
+  if (k % 16 != 0) return set_error(FMOE_ERR_INVALID_ARG, "k must be a multiple of 16");
+  if (experts > 1 && offsets == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "several experts need offsets");
+  const long long row_tiles = static_cast<long long>(m) / 16 + experts;
+  if (static_cast<long long>(experts) * n > 0x7fffff00ll || row_tiles * (n / 128 + 1) * experts > 0x7fffffffll ||
+      m > 0x7fffff00)
+    return set_error(FMOE_ERR_UNSUPPORTED, "more rows, features or tiles than 32-bit tile numbers hold");
+  if (m > 0 && (a == nullptr || a_scale == nullptr || w == nullptr || w_scale == nullptr))
+    return set_error(FMOE_ERR_INVALID_ARG, "both operands and their scales are required");
+  if (misaligned(a, 16) || misaligned(w, 16)) return set_error(FMOE_ERR_INVALID_ARG, "operands must be 16-byte aligned");
+  if (misaligned(a_scale, 4) || misaligned(w_scale, 4) || misaligned(offsets, 4))
+    return set_error(FMOE_ERR_INVALID_ARG, "scales and offsets must be 4-byte aligned");
+  return FMOE_OK;
+}
+
+ProductParams product_params(int m, int n, int k, int experts, const int32_t* offsets, int tile_n, int device) {
+  ProductParams p{};
+  p.m = m; p.n = n; p.k = k;
+  p.kblocks = blocks_of(k); p.nblocks = blocks_of(n);
+  p.experts = experts;
+  p.offsets = offsets;
+  p.tiles_n = (n + tile_n - 1) / tile_n;
+  p.spin_limit = facts(device).spin_limit;
+  return p;
+}
+
+int grid_for(const ProductParams& p, int tile_m, int device) {
+  const long long most = (static_cast<long long>((p.m + tile_m - 1) / tile_m) + (p.experts > 1 ? p.experts : 0)) * p.tiles_n;
+  const int sms = facts(device).sms;
+  return static_cast<int>(most < sms ? most : sms);
+}
+
+}  // namespace
+
+int sm_count(int device) { return facts(device).sms; }
+
+}  // namespace fmoe::fp8
+
+using namespace fmoe;
+using namespace fmoe::fp8;
+
+extern "C" {
+
+int fmoe_fp8_matmul(const fmoe_fp8_matmul_args* a, void* stream) {
+  if (a == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "arguments are null");
+  int rc = check_product(a->a, a->a_scale, a->w, a->w_scale, a->offsets, a->m, a->n, a->k, a->num_experts, a->device_id);
+  if (rc != FMOE_OK) return rc;
+  if (a->data_type != FMOE_DT_BF16 && a->data_type != FMOE_DT_FP16 && a->data_type != FMOE_DT_FP32)
+    return set_error(FMOE_ERR_UNSUPPORTED, "the 8-bit product is written as BF16, FP16 or FP32");
+  const int eb = element_bytes(a->data_type);
+  if (a->m == 0) return FMOE_OK;
+  if (a->out == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "out is required");
+  if (misaligned(a->out, eb)) return set_error(FMOE_ERR_INVALID_ARG, "out must be aligned to its type");
+  OnDevice on(a->device_id);
+  if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));
+  ProductParams p = product_params(a->m, a->n, a->k, a->num_experts, a->offsets, 256, a->device_id);
+  p.a_scale = a->a_scale;
+  p.w_scale[0] = a->w_scale;
+  p.out = a->out;
+  p.wide = !misaligned(a->out, 32) && (static_cast<size_t>(a->n) * eb) % 32 == 0;
+  CUtensorMap maps[3];
+  rc = make_byte_map(&maps[0], a->a, a->m, a->k, 128);
+  if (rc == FMOE_OK) rc = make_byte_map(&maps[1], a->w, static_cast<uint64_t>(a->num_experts) * a->n, a->k, 128);
+  if (rc != FMOE_OK) return rc;
+  maps[2] = maps[1];
+  const int grid = grid_for(p, 128, a->device_id);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->data_type == FMOE_DT_BF16) return launch_product_of<__nv_bfloat16>(p, maps, grid, a->device_id, st);
+  if (a->data_type == FMOE_DT_FP16) return launch_product_of<__half>(p, maps, grid, a->device_id, st);
+  return launch_product_of<float>(p, maps, grid, a->device_id, st);
+}
+
+int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* a, void* stream) {
+  if (a == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "arguments are null");
+  int rc = check_product(a->a, a->a_scale, a->up, a->up_scale, a->offsets, a->m, a->ffn_size, a->k, a->num_experts,
+                         a->device_id);
+  if (rc != FMOE_OK) return rc;
+  if (a->ffn_size % 16 != 0) return set_error(FMOE_ERR_INVALID_ARG, "ffn_size must be a multiple of 16");
+  if (a->act_type < FMOE_ACT_IDENTITY || a->act_type > FMOE_ACT_RELU)
+    return set_error(FMOE_ERR_INVALID_ARG, "unknown act_type");
+  if (a->m == 0) return FMOE_OK;
+  if (a->q == nullptr || a->scale == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "q and scale are required");
+  if (misaligned(a->q, 16) || misaligned(a->up_v, 16)) return set_error(FMOE_ERR_INVALID_ARG, "q and up_v must be 16-byte aligned");
+  if (misaligned(a->scale, 4) || misaligned(a->up_v_scale, 4))
+    return set_error(FMOE_ERR_INVALID_ARG, "scales must be 4-byte aligned");
+  if (a->up_v != nullptr && a->up_v_scale == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "up_v needs its scales");
+  OnDevice on(a->device_id);
+  if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));
+  ProductParams p = product_params(a->m, a->ffn_size, a->k, a->num_experts, a->offsets, 128, a->device_id);
+  p.a_scale = a->a_scale;
+  p.w_scale[0] = a->up_scale;
+  p.w_scale[1] = a->up_v_scale;
+  p.out = a->q;
+  p.out_scale = a->scale;
+  p.act = a->act_type;
+  p.has_v = a->up_v != nullptr;
+  CUtensorMap maps[3];
+  const uint64_t w_rows = static_cast<uint64_t>(a->num_experts) * a->ffn_size;
+  rc = make_byte_map(&maps[0], a->a, a->m, a->k, 128);
+  if (rc == FMOE_OK) rc = make_byte_map(&maps[1], a->up, w_rows, a->k, 128);
+  if (rc == FMOE_OK) rc = make_byte_map(&maps[2], a->up_v != nullptr ? a->up_v : a->up, w_rows, a->k, 128);
+  if (rc != FMOE_OK) return rc;
+  return launch_product_of<Codes>(p, maps, grid_for(p, 128, a->device_id), a->device_id, static_cast<cudaStream_t>(stream));
+}
+
+int fmoe_fp8_last_status(int32_t device_id, void* stream, fmoe_status* out) {
+  if (out == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "out is null");
+  if (device_id < 0 || device_id >= kMaxDevices) return set_error(FMOE_ERR_INVALID_ARG, "device_id out of range");
+  OnDevice on(device_id);
+  cudaError_t e = on.err;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const fmoe_status none{};
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(out, g_status, sizeof(fmoe_status), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && out->code != FMOE_OK) {
+    e = cudaMemcpyToSymbolAsync(g_status, &none, sizeof(none), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("fmoe_fp8_last_status: ") + cudaGetErrorString(e));
+  return FMOE_OK;
+}
+
+}  // extern "C"

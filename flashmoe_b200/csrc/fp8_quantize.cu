@@ -1,0 +1,187 @@
+// Quantisation to e4m3 with a scale per block: rows in 1 x 128 blocks (optionally laid out by
+// expert on the way), weights in 128 x 128 blocks.  Each value is read once and kept in registers
+// between the maximum and the rounding.
+#include "fp8.cuh"
+
+namespace fmoe::fp8 {
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+struct QuantizeParams {
+  const void* x;
+  unsigned char* q;
+  float* scale;
+  const int32_t* positions;   // rows: [rows, copies] or null
+  int copies;
+  int rows, cols;
+  int row_blocks, col_blocks;
+};
+
+// 16 consecutive values as loaded.
+template <typename T>
+struct Raw16 {
+  static constexpr int kPieces = static_cast<int>(sizeof(T));
+  static constexpr int kPer = 16 / sizeof(T);
+  uint4 u[kPieces];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) u[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void values(float (&f)[16]) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      float part[kPer];
+      unpack16<T>(u[i], part);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) f[i * kPer + j] = part[j];
+    }
+  }
+  __device__ __forceinline__ uint32_t amax() const {
+    float f[16];
+    values(f);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, abs_bits(f[i]));
+    return m;
+  }
+  __device__ __forceinline__ uint4 codes(const Quantizer& z) const {
+    float f[16];
+    values(f);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = to_e4m3x4(z.scaled(f[4 * i]), z.scaled(f[4 * i + 1]), z.scaled(f[4 * i + 2]), z.scaled(f[4 * i + 3]));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// Eight threads a block of 128, sixteen values each.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams p) {
+  const long long block = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 3;
+  const int sub = threadIdx.x & 7;
+  const long long row = block / p.col_blocks;
+  const int cb = static_cast<int>(block - row * p.col_blocks), col = cb * kBlock + sub * 16;
+  const bool in = row < p.rows && col < p.cols;   // (cols is a multiple of 16)
+  Raw16<T> raw;
+  raw.zero();
+  if (in) raw.load(static_cast<const T*>(p.x) + row * p.cols + col);
+  uint32_t m = raw.amax();
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  const float amax = __uint_as_float(m);
+  const uint4 codes = raw.codes(Quantizer(amax));
+  if (row >= p.rows) return;
+  for (int j = 0; j < p.copies; ++j) {
+    long long to = row;
+    if (p.positions != nullptr) {
+      to = __ldg(p.positions + row * p.copies + j);
+      if (to < 0 || to >= static_cast<long long>(p.rows) * p.copies) continue;
+    }
+    if (in) *reinterpret_cast<uint4*>(p.q + to * p.cols + col) = codes;
+    if (sub == 0) p.scale[to * p.col_blocks + cb] = block_scale(amax);
+  }
+}
+
+// One CTA a block of 128 x 128: a pass takes 32 rows, eight threads each; four passes stay in registers.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_weights_kernel(const QuantizeParams p) {
+  __shared__ uint32_t s_max[8];
+  const long long matrix = blockIdx.y;
+  const int rb = blockIdx.x / p.col_blocks, cb = blockIdx.x - rb * p.col_blocks;
+  const int row0 = rb * kBlock + (threadIdx.x >> 3), col = cb * kBlock + (threadIdx.x & 7) * 16;
+  const size_t base = static_cast<size_t>(matrix) * p.rows * p.cols + col;
+  Raw16<T> raw[4];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    raw[i].zero();
+    if (row0 + 32 * i < p.rows && col < p.cols)
+      raw[i].load(static_cast<const T*>(p.x) + base + static_cast<size_t>(row0 + 32 * i) * p.cols);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, raw[i].amax());
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, s_max[i]);
+  const float amax = __uint_as_float(m);
+  const Quantizer z(amax);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (row0 + 32 * i < p.rows && col < p.cols)
+      *reinterpret_cast<uint4*>(p.q + base + static_cast<size_t>(row0 + 32 * i) * p.cols) = raw[i].codes(z);
+  }
+  if (threadIdx.x == 0) p.scale[(matrix * p.row_blocks + rb) * p.col_blocks + cb] = block_scale(amax);
+}
+
+template <typename T>
+cudaError_t launch(const QuantizeParams& p, int block_rows, int matrices, cudaStream_t stream) {
+  if (block_rows == 1) {
+    const long long threads = static_cast<long long>(p.rows) * p.col_blocks * 8;
+    quantize_rows_kernel<T><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, stream>>>(p);
+  } else {
+    quantize_weights_kernel<T><<<dim3(static_cast<unsigned>(p.row_blocks * p.col_blocks), matrices), 256, 0, stream>>>(p);
+  }
+  ++g_launches;
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace fmoe::fp8
+
+extern "C" int fmoe_fp8_quantize(const fmoe_fp8_quantize_args* a, void* stream) {
+  using namespace fmoe;
+  using namespace fmoe::fp8;
+  if (a == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "arguments are null");
+  if (a->rows < 0 || a->num_matrices < 0 || a->cols < 1)
+    return set_error(FMOE_ERR_INVALID_ARG, "rows and num_matrices must not be negative, cols must be positive");
+  if (a->cols % 16 != 0) return set_error(FMOE_ERR_INVALID_ARG, "cols must be a multiple of 16");
+  if (a->block_rows != 1 && a->block_rows != kBlock)
+    return set_error(FMOE_ERR_INVALID_ARG, "block_rows must be 1 (rows) or 128 (weights)");
+  if (a->data_type != FMOE_DT_BF16 && a->data_type != FMOE_DT_FP16 && a->data_type != FMOE_DT_FP32)
+    return set_error(FMOE_ERR_UNSUPPORTED, "BF16, FP16 and FP32 can be quantised");
+  if (a->device_id < 0 || a->device_id >= kMaxDevices) return set_error(FMOE_ERR_INVALID_ARG, "device_id out of range");
+  if (a->positions != nullptr && (a->block_rows != 1 || a->num_matrices != 1))
+    return set_error(FMOE_ERR_INVALID_ARG, "positions go with block_rows 1 and one matrix");
+  if (a->copies < 1 || (a->positions == nullptr && a->copies != 1))
+    return set_error(FMOE_ERR_INVALID_ARG, "copies must be positive, and 1 without positions");
+  if (static_cast<long long>(a->rows) * a->copies > 0x7fffffffll)
+    return set_error(FMOE_ERR_UNSUPPORTED, "rows * copies must fit 32 bits");
+  if (a->rows == 0 || a->num_matrices == 0) return FMOE_OK;
+  if (a->x == nullptr || a->q == nullptr || a->scale == nullptr)
+    return set_error(FMOE_ERR_INVALID_ARG, "x, q and scale are required");
+  if (misaligned(a->x, 16) || misaligned(a->q, 16)) return set_error(FMOE_ERR_INVALID_ARG, "x and q must be 16-byte aligned");
+  if (misaligned(a->scale, 4) || misaligned(a->positions, 4))
+    return set_error(FMOE_ERR_INVALID_ARG, "scale and positions must be 4-byte aligned");
+  QuantizeParams p{a->x, static_cast<unsigned char*>(a->q), a->scale, a->positions, a->copies, a->rows, a->cols, 0, 0};
+  p.row_blocks = a->block_rows == 1 ? a->rows : blocks_of(a->rows);
+  p.col_blocks = blocks_of(a->cols);
+  int matrices = a->num_matrices;
+  if (a->block_rows == 1) {   // rows of several matrices are just more rows
+    if (static_cast<long long>(a->rows) * matrices > 0x7fffffffll)
+      return set_error(FMOE_ERR_UNSUPPORTED, "rows * num_matrices must fit 32 bits");
+    p.rows *= matrices;
+    p.row_blocks = p.rows;
+    matrices = 1;
+    if (static_cast<long long>(p.rows) * p.col_blocks * 8 / 256 >= 0x7fffffffll)
+      return set_error(FMOE_ERR_UNSUPPORTED, "more blocks than a grid holds");
+  } else if (matrices > 65535 || static_cast<long long>(p.row_blocks) * p.col_blocks > 0x7fffffffll) {
+    return set_error(FMOE_ERR_UNSUPPORTED, "at most 65535 matrices, and blocks of one must fit 32 bits");
+  }
+  OnDevice on(a->device_id);
+  if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (a->data_type == FMOE_DT_BF16) e = launch<__nv_bfloat16>(p, a->block_rows, matrices, st);
+  else if (a->data_type == FMOE_DT_FP16) e = launch<__half>(p, a->block_rows, matrices, st);
+  else e = launch<float>(p, a->block_rows, matrices, st);
+  if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("quantize launch: ") + cudaGetErrorString(e));
+  return FMOE_OK;
+}

@@ -1,0 +1,511 @@
+// Routing from logits: scores, choice, weights, and the order of the (token, choice) pairs by expert.
+//
+// Choosing is one warp per token with the row of scores in registers; ordering is a stable counting
+// sort of the pairs by expert, by one cluster of CTAs whose histograms meet in distributed shared
+// memory, so neither step needs scratch memory or atomics whose order could show.
+//
+// Which experts are chosen hangs on comparisons, and fp32 scores carry an error: where two of the
+// scores that a decision hangs on are closer than twice that error, the token's row is decided again
+// in 64 bits.  Without a bias the scores are never compared at all: softmax and sigmoid keep the
+// order of the logits, so the logits, which are exact, are (inside a group too).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cfloat>
+
+#include "fp8.cuh"
+
+namespace fmoe {
+namespace {
+
+constexpr int kMaxExperts = 1024, kMaxTopK = 32, kMaxGroups = 32;
+constexpr int kMaxDevices = 64;
+constexpr unsigned kAll = 0xffffffffu;
+
+struct SelectParams {
+  const void* logits;
+  const float* bias;
+  int32_t* ids;
+  float* weights;
+  int32_t* counts;
+  int32_t* offsets;
+  int32_t* positions;
+  TokenSlot* table;     // of an MoE context, or null
+  Route* routes;
+  int capacity, round_ec;
+  int S, E, k, dtype, score, groups, top_groups, group_max, renormalize;
+  float scale;
+};
+
+// ---- choosing ---------------------------------------------------------------------------------------
+
+// A masked expert (-infinity or NaN) orders below every other; +infinity is the largest finite number.
+__device__ __forceinline__ float sane(float x) { return x == x ? fminf(x, FLT_MAX) : -INFINITY; }
+
+__device__ __forceinline__ float logit_at(const SelectParams& p, size_t i) {
+  float x;
+  if (p.dtype == FMOE_DT_FP32) x = __ldg(static_cast<const float*>(p.logits) + i);
+  else if (p.dtype == FMOE_DT_BF16) x = __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.logits) + i));
+  else x = __half2float(__ldg(static_cast<const __half*>(p.logits) + i));
+  return sane(x);
+}
+
+// An unsigned number that orders like the value (+0 and -0 alike); 0 is left for "nothing".
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+template <typename F>
+__device__ __forceinline__ F exp_of(F x) {
+  if constexpr (sizeof(F) == 8) return exp(x); else return expf(x);
+}
+// exp(l - largest) or sigmoid(l); 0 for a masked logit
+template <typename F>
+__device__ __forceinline__ F raw_score(F l, F largest, int score) {
+  if (l == -INFINITY) return 0;
+  if (score == FMOE_SCORE_SOFTMAX) return exp_of<F>(l - largest);
+  if (sizeof(F) == 8 || l >= 0) return F(1) / (F(1) + exp_of<F>(-l));
+  const F e = exp_of<F>(l);   // (exp(-l) would overflow fp32 from -89 on)
+  return e / (F(1) + e);
+}
+
+template <typename F>
+__device__ __forceinline__ F warp_sum(F v) {
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(kAll, v, d);
+  return v;
+}
+template <typename F>
+__device__ __forceinline__ F warp_max(F v) {
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) {
+    const F o = __shfl_xor_sync(kAll, v, d);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+// A group's score from its experts' values in shared memory: teams of lanes, one a group, walk the
+// values and keep the two largest.  Lane g < groups leaves with group g's score.
+template <typename F>
+__device__ __forceinline__ F group_score(const F* row, int E, int groups, bool largest_only, int lane) {
+  int team = 32;
+  while (team * groups > 32) team >>= 1;
+  const int g = lane / team, sub = lane - g * team, size = E / groups;
+  F a = -INFINITY, b = -INFINITY;   // the largest two
+  if (g < groups) {
+    for (int j = sub; j < size; j += team) {
+      const F v = row[g * size + j];
+      if (v > a) { b = a; a = v; } else if (v > b) { b = v; }
+    }
+  }
+  for (int d = 1; d < team; d <<= 1) {
+    const F oa = __shfl_xor_sync(kAll, a, d), ob = __shfl_xor_sync(kAll, b, d);
+    if (oa > a) { b = a > ob ? a : ob; a = oa; } else { b = oa > b ? oa : b; }
+  }
+  const F s = largest_only || b == -INFINITY ? a : a + b;   // (masked experts add nothing)
+  return __shfl_sync(kAll, s, (lane * team) & 31);
+}
+
+// Which groups stay, as bits; `gap` is how far the worst that stays lies above the best that goes.
+template <typename F>
+__device__ __forceinline__ uint32_t kept_groups(F mine, int groups, int top_groups, int lane, F& worst_kept, F& best_gone) {
+  int before = 0;
+  for (int g = 0; g < groups; ++g) {
+    const F o = __shfl_sync(kAll, mine, g);
+    before += o > mine || (o == mine && g < lane);
+  }
+  const bool stays = lane < groups && before < top_groups;
+  worst_kept = -warp_max<F>(stays ? -mine : F(-INFINITY));
+  best_gone = warp_max<F>(lane < groups && !stays ? mine : F(-INFINITY));
+  return __ballot_sync(kAll, stays);
+}
+
+// Bits i of the experts lane + 32 i that exist and whose group stays.
+template <int V>
+__device__ __forceinline__ uint32_t alive_bits(int E, int groups, uint32_t kept, int lane) {
+  uint32_t alive = 0;
+  const float per = static_cast<float>(groups) / static_cast<float>(E);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane + 32 * i;
+    // (e + 1/2) / size lies at least 1/2048 from a whole number, fp32 is exact to far less
+    const int g = static_cast<int>((static_cast<float>(e) + 0.5f) * per);
+    if (e < E && (groups == 1 || (kept >> g & 1))) alive |= 1u << i;
+  }
+  return alive;
+}
+
+// The row decided in 64 bits; lane j < k leaves with the j-th choice.
+template <int V>
+__device__ __noinline__ int choose_exactly(const SelectParams& p, size_t row, int lane, double* shared_row) {
+  double c[V];
+  double top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane + 32 * i;
+    c[i] = e < p.E ? static_cast<double>(logit_at(p, row + e)) : static_cast<double>(-INFINITY);
+    top = c[i] > top ? c[i] : top;
+  }
+  top = warp_max<double>(top);
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const bool masked = c[i] == -INFINITY;
+    c[i] = raw_score<double>(c[i], top, p.score);
+    sum += c[i];
+    if (masked) c[i] = -INFINITY;
+  }
+  sum = warp_sum<double>(sum);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane + 32 * i;
+    if (p.score == FMOE_SCORE_SOFTMAX && sum > 0.0) c[i] /= sum;
+    if (p.bias != nullptr && e < p.E) c[i] += static_cast<double>(sane(__ldg(p.bias + e)));
+  }
+  uint32_t kept = kAll;
+  if (p.groups > 1) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (lane + 32 * i < p.E) shared_row[lane + 32 * i] = c[i];
+    __syncwarp();
+    double worst, best;
+    kept = kept_groups<double>(group_score<double>(shared_row, p.E, p.groups, p.group_max, lane), p.groups, p.top_groups,
+                               lane, worst, best);
+  }
+  if (p.bias == nullptr) {   // the groups were the question
+#pragma unroll
+    for (int i = 0; i < V; ++i) c[i] = lane + 32 * i < p.E ? static_cast<double>(logit_at(p, row + lane + 32 * i)) : 0.0;
+  }
+  uint32_t alive = alive_bits<V>(p.E, p.groups, kept, lane);
+  int mine = 0;
+  for (int r = 0; r < p.k; ++r) {
+    double best = -INFINITY;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if ((alive >> i & 1) && (at == 0x7fffffff || c[i] > best)) { best = c[i]; at = lane + 32 * i; }
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) {
+      const double o = __shfl_xor_sync(kAll, best, d);
+      const int oa = __shfl_xor_sync(kAll, at, d);
+      if (oa != 0x7fffffff && (at == 0x7fffffff || o > best || (o == best && oa < at))) { best = o; at = oa; }
+    }
+    if (lane == (at & 31)) alive &= ~(1u << (at >> 5));
+    if (lane == r) mine = at;
+  }
+  return mine;
+}
+
+// One token by one warp: ids and weights.  shared_row: E doubles, used with groups only.
+template <int V>
+__device__ __forceinline__ void select_token(const SelectParams& p, int token, int lane, double* shared_row) {
+  const size_t row = static_cast<size_t>(token) * p.E;
+  float v[V];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane + 32 * i;
+    v[i] = e < p.E ? logit_at(p, row + e) : -INFINITY;
+    top = fmaxf(top, v[i]);
+  }
+  top = warp_max<float>(top);
+  const bool softmax = p.score == FMOE_SCORE_SOFTMAX, by_score = p.bias != nullptr || p.groups > 1;
+  float sum = 1.0f;
+  float c[V];   // what is compared
+  if (by_score || (softmax && !p.renormalize)) {
+    float part = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      c[i] = raw_score<float>(v[i], top, p.score);
+      part += c[i];
+    }
+    if (softmax) sum = warp_sum<float>(part);
+  }
+  // how far a computed score may be from the true one: sigmoid takes an exp of 1 ulp and two roundings;
+  // softmax also the rounding of l - max (at most 2^-25 of the largest score: x exp(-x) < 1/2) and a sum of
+  // up to 37 additions in a row, all relative to the score, which is at most exp(0) / sum
+  const float error = softmax ? 0x1p-18f / (sum > 0.0f ? sum : 1.0f) : 0x1p-21f;
+  bool unsure = false;
+  uint32_t kept = kAll;
+  if (by_score) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int e = lane + 32 * i;
+      if (softmax && sum > 0.0f) c[i] = c[i] / sum;
+      if (v[i] == -INFINITY) c[i] = -INFINITY;
+      if (p.bias != nullptr && e < p.E) c[i] += sane(__ldg(p.bias + e));
+    }
+    if (p.groups > 1) {
+      float* shared = reinterpret_cast<float*>(shared_row);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (lane + 32 * i < p.E) shared[lane + 32 * i] = c[i];
+      __syncwarp();
+      float worst, best;
+      kept = kept_groups<float>(group_score<float>(shared, p.E, p.groups, p.group_max, lane), p.groups, p.top_groups, lane,
+                                worst, best);
+      if (p.top_groups < p.groups)
+        unsure = worst - best <= 4.0f * error + 0x1p-21f * (fabsf(worst) + fabsf(best));
+    }
+  }
+  const bool by_logit = p.bias == nullptr;
+  if (by_logit) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) c[i] = v[i];
+  }
+  uint32_t alive = alive_bits<V>(p.E, p.groups, kept, lane);
+  uint32_t best = 0;
+  int at = 0x7fffffff;
+  auto find_best = [&] {
+    best = 0;
+    at = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint32_t key = order_key(c[i]);
+      if ((alive >> i & 1) && key > best) { best = key; at = lane + 32 * i; }
+    }
+  };
+  find_best();
+  int mine = 0;
+  float last = 0.0f;
+  const int rounds = by_logit ? p.k : p.k + 1;   // one more round shows how near the first unchosen one is
+  for (int r = 0; r < rounds; ++r) {
+    const uint32_t key = __reduce_max_sync(kAll, best);
+    if (key == 0) break;                         // every expert is taken (the extra round)
+    const int e = __reduce_min_sync(kAll, best == key ? at : 0x7fffffff);
+    if (!by_logit) {
+      const float now = key_value(key);
+      if (r > 0 && last - now <= 2.0f * error + 0x1p-23f * fmaxf(fabsf(last), fabsf(now))) unsure = true;
+      last = now;
+    }
+    if (lane == r && r < p.k) mine = e;
+    if (lane == (e & 31)) {
+      alive &= ~(1u << (e >> 5));
+      find_best();
+    }
+  }
+  if (unsure) mine = choose_exactly<V>(p, row, lane, shared_row);   // (the same for the whole warp)
+  const float l = lane < p.k ? logit_at(p, row + mine) : -INFINITY;
+  // (shares among the chosen do not depend on the largest of all, which may be far above theirs)
+  float s = raw_score<float>(l, p.renormalize ? warp_max<float>(l) : top, p.score);
+  if (softmax && !p.renormalize && sum > 0.0f) s = s / sum;
+  if (p.renormalize) {
+    const float total = warp_sum<float>(s);
+    s = total > 0.0f ? s / total : 0.0f;
+  }
+  if (lane < p.k) {
+    p.ids[static_cast<size_t>(token) * p.k + lane] = mine;
+    p.weights[static_cast<size_t>(token) * p.k + lane] = s * p.scale;
+  }
+}
+
+template <int V>
+__global__ void __launch_bounds__(256) select_kernel(const SelectParams p) {
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int token = blockIdx.x * 8 + warp;
+  if (token < p.S) select_token<V>(p, token, lane, reinterpret_cast<double*>(s_raw) + static_cast<size_t>(warp) * p.E);
+}
+
+// ---- ordering ---------------------------------------------------------------------------------------
+
+constexpr int kOrderThreads = 512, kOrderWarps = kOrderThreads / 32, kOrderCtas = 8;
+
+// Stable counting sort of the pairs by expert: the CTAs of one cluster take consecutive runs of pairs, their
+// warps consecutive runs of those.  Pass one counts, pass two hands out places in the same order.
+// A token's experts differ, so pairs in order are tokens in order within an expert.
+__global__ void __launch_bounds__(kOrderThreads) order_kernel(const SelectParams p) {
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  const int E = p.E, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* hist = reinterpret_cast<int*>(s_raw);      // [warps][E]: counts, then places already handed out
+  int* total = hist + kOrderWarps * E;            // [E]: this CTA's pairs
+  int* start = total + E;                         // [E]: first row of the expert, then of this CTA's share
+  int* before = start + E;                        // [E]: this CTA's first slot within the expert
+  const int ctas = gridDim.x, cta = blockIdx.x;   // the grid is one cluster
+  for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) hist[i] = 0;
+  __syncthreads();
+  const long long pairs = static_cast<long long>(p.S) * p.k;
+  const long long workers = static_cast<long long>(ctas) * kOrderWarps;
+  const long long share = ((pairs + workers - 1) / workers + 31) & ~31ll;
+  const long long first = min(pairs, (static_cast<long long>(cta) * kOrderWarps + warp) * share);
+  const long long end = min(pairs, first + share);
+  int* mine = hist + warp * E;
+  for (long long i = first + lane; i < end; i += 32) atomicAdd(mine + __ldg(p.ids + i), 1);
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kOrderThreads) {
+    int sum = 0;
+    for (int w = 0; w < kOrderWarps; ++w) {
+      const int c = hist[w * E + e];
+      hist[w * E + e] = sum;
+      sum += c;
+    }
+    total[e] = sum;
+  }
+  if (ctas > 1) ptx::cluster_sync_all(); else __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kOrderThreads) {
+    int all = 0, lower = 0;
+    for (int c = 0; c < ctas; ++c) {
+      int n;
+      if (ctas > 1) asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(n) : "r"(ptx::map_to_cta(total + e, c)) : "memory");
+      else n = total[e];
+      if (c < cta) lower += n;
+      all += n;
+    }
+    before[e] = lower;
+    start[e] = all;
+    if (cta == 0) p.counts[e] = all;
+  }
+  __syncthreads();
+  if (warp == 0) {   // exclusive sum over the experts
+    int carry = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane, own = e < E ? start[e] : 0;
+      int sum = own;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(kAll, sum, d);
+        if (lane >= d) sum += o;
+      }
+      if (e < E) {
+        start[e] = carry + sum - own;
+        if (cta == 0 && p.offsets != nullptr) p.offsets[e] = carry + sum - own;
+      }
+      carry += __shfl_sync(kAll, sum, 31);
+    }
+    if (cta == 0 && lane == 0 && p.offsets != nullptr) p.offsets[E] = carry;
+  }
+  __syncthreads();
+  if (p.positions != nullptr || p.table != nullptr) {
+    for (long long i0 = first; i0 < end; i0 += 32) {
+      const long long i = i0 + lane;
+      const int e = i < end ? __ldg(p.ids + i) : -1;
+      const unsigned same = __match_any_sync(kAll, e);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      int slot = 0;
+      if (e >= 0) slot = before[e] + mine[e] + rank;
+      __syncwarp();
+      if (e >= 0 && rank == 0) mine[e] += __popc(same);
+      __syncwarp();
+      if (e >= 0) {
+        if (p.positions != nullptr) p.positions[i] = start[e] + slot;
+        if (p.table != nullptr) {
+          const float w = __ldg(p.weights + i);
+          if (slot < p.capacity)
+            p.table[static_cast<size_t>(e) * p.round_ec + slot] = TokenSlot{static_cast<uint32_t>(i / p.k), w};
+          p.routes[i] = Route{e, slot, w, 0};
+        }
+      }
+    }
+  }
+  if (ctas > 1) ptx::cluster_sync_all();   // no CTA leaves while another reads its totals
+}
+
+size_t order_smem(int E) { return static_cast<size_t>(kOrderWarps + 3) * E * sizeof(int); }
+
+cudaError_t launch_order(const SelectParams& p, cudaStream_t stream) {
+  const size_t smem = order_smem(p.E);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+  }
+  const long long pairs = static_cast<long long>(p.S) * p.k;
+  const int ctas = pairs <= 4 * kOrderThreads ? 1 : kOrderCtas;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kOrderThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  ++g_launches;
+  return cudaLaunchKernelEx(&cfg, order_kernel, p);
+}
+
+template <int V>
+cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
+  if (p.S > 0) {
+    const size_t smem = p.groups > 1 ? 8 * static_cast<size_t>(p.E) * sizeof(double) : 0;
+    if (smem > 48 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(select_kernel<V>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      if (e != cudaSuccess) return e;
+    }
+    select_kernel<V><<<(p.S + 7) / 8, 256, smem, stream>>>(p);
+    ++g_launches;
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  return launch_order(p, stream);
+}
+
+int check(const fmoe_select_args* a) {
+  if (a == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "arguments are null");
+  if (a->num_tokens < 0) return set_error(FMOE_ERR_INVALID_ARG, "num_tokens must not be negative");
+  if (a->num_experts < 1 || a->num_experts > kMaxExperts)
+    return set_error(FMOE_ERR_INVALID_ARG, "num_experts must be between 1 and " + std::to_string(kMaxExperts));
+  if (a->num_groups < 1 || a->num_groups > kMaxGroups || a->num_experts % a->num_groups != 0)
+    return set_error(FMOE_ERR_INVALID_ARG, "num_groups must divide num_experts and be at most " + std::to_string(kMaxGroups));
+  if (a->top_groups < 1 || a->top_groups > a->num_groups)
+    return set_error(FMOE_ERR_INVALID_ARG, "top_groups must be between 1 and num_groups");
+  if (a->top_k < 1 || a->top_k > kMaxTopK || a->top_k > a->top_groups * (a->num_experts / a->num_groups))
+    return set_error(FMOE_ERR_INVALID_ARG, "top_k must not exceed the experts of top_groups groups (or 32)");
+  if (a->score != FMOE_SCORE_SOFTMAX && a->score != FMOE_SCORE_SIGMOID)
+    return set_error(FMOE_ERR_INVALID_ARG, "unknown score");
+  if (a->group_score != FMOE_GROUP_TOP2 && a->group_score != FMOE_GROUP_MAX)
+    return set_error(FMOE_ERR_INVALID_ARG, "unknown group_score");
+  if (a->data_type != FMOE_DT_BF16 && a->data_type != FMOE_DT_FP16 && a->data_type != FMOE_DT_FP32)
+    return set_error(FMOE_ERR_UNSUPPORTED, "logits are BF16, FP16 or FP32");
+  if (a->device_id < 0 || a->device_id >= kMaxDevices) return set_error(FMOE_ERR_INVALID_ARG, "device_id out of range");
+  if (static_cast<long long>(a->num_tokens) * a->top_k > 0x7fffffffll)
+    return set_error(FMOE_ERR_UNSUPPORTED, "num_tokens * top_k must fit 32 bits");
+  if (a->expert_counts == nullptr || (a->num_tokens > 0 && (a->logits == nullptr || a->ids == nullptr || a->weights == nullptr)))
+    return set_error(FMOE_ERR_INVALID_ARG, "logits, ids, weights and expert_counts are required");
+  if (fp8::misaligned(a->logits, fp8::element_bytes(a->data_type)) || fp8::misaligned(a->bias, 4) || fp8::misaligned(a->ids, 4) ||
+      fp8::misaligned(a->weights, 4) || fp8::misaligned(a->expert_counts, 4) || fp8::misaligned(a->offsets, 4) ||
+      fp8::misaligned(a->positions, 4))
+    return set_error(FMOE_ERR_INVALID_ARG, "every array must be aligned to its type");
+  return FMOE_OK;
+}
+
+}  // namespace
+}  // namespace fmoe
+
+extern "C" int fmoe_router_select(fmoe_ctx* moe, const fmoe_select_args* a, void* stream) {
+  using namespace fmoe;
+  int rc = check(a);
+  if (rc != FMOE_OK) return rc;
+  SelectParams p{};
+  if (moe != nullptr) {
+    rc = routing_targets(moe, a->num_tokens, a->num_experts, a->top_k, a->device_id, &p.table, &p.routes, &p.capacity, &p.round_ec);
+    if (rc != FMOE_OK) return rc;
+  }
+  p.logits = a->logits; p.bias = a->bias; p.ids = a->ids; p.weights = a->weights;
+  p.counts = a->expert_counts; p.offsets = a->offsets; p.positions = a->positions;
+  p.S = a->num_tokens; p.E = a->num_experts; p.k = a->top_k; p.dtype = a->data_type; p.score = a->score;
+  p.groups = a->top_groups == a->num_groups ? 1 : a->num_groups;   // every group stays: as if there were none
+  p.top_groups = p.groups == 1 ? 1 : a->top_groups;
+  p.group_max = a->group_score == FMOE_GROUP_MAX;
+  p.renormalize = a->renormalize != 0; p.scale = a->scale;
+  fp8::OnDevice on(a->device_id);
+  if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (p.E <= 32) e = launch_select<1>(p, st);
+  else if (p.E <= 64) e = launch_select<2>(p, st);
+  else if (p.E <= 128) e = launch_select<4>(p, st);
+  else if (p.E <= 256) e = launch_select<8>(p, st);
+  else if (p.E <= 512) e = launch_select<16>(p, st);
+  else e = launch_select<32>(p, st);
+  if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("select launch: ") + cudaGetErrorString(e));
+  return FMOE_OK;
+}

@@ -3,9 +3,11 @@
 from __future__ import annotations
 
 import ctypes as C
+from enum import IntEnum
+from typing import Optional
 
 from . import _native as N
-from .jit import ContextHandle, InitArgs, _get_compiled
+from .jit import ContextHandle, DataType, InitArgs, _get_compiled
 
 
 class _RouterModule:
@@ -63,3 +65,50 @@ def forward(router_handle: ContextHandle, flash_handle: ContextHandle, arg: Rout
 
 def finalize(handle: ContextHandle, stream_ptr: int) -> None:
     handle.mod.finalize(handle.context, stream_ptr)
+
+
+# ---- routing from logits (an addition of this package) ------------------------------------------
+
+class Score(IntEnum):
+    """What a logit becomes."""
+    SOFTMAX = 0
+    SIGMOID = 1
+
+
+class GroupScore(IntEnum):
+    """What a group of experts is ranked by: the sum of its two largest scores, or its largest."""
+    TOP2 = 0
+    MAX = 1
+
+
+class SelectArgs:
+    """Arguments of `select`.  Device addresses: logits [S, E] of `data_type` (BF16, FP16 or FP32);
+    out: ids [S, k] int32 (descending by score, ties to the lower id), weights [S, k] fp32,
+    expert_counts [E] int32, and, where not 0, offsets [E + 1] int32 (their exclusive sums) and
+    positions [S, k] int32 (the row of every pair when the pairs are ordered by expert).
+
+    `bias` ([E] fp32, 0 = none) is added to the scores for the choice only.  With `num_groups` > 1 the
+    experts fall into that many equal runs, of which the `top_groups` best stay.  The weights are the
+    chosen experts' scores, divided by their sum if `renormalize`, times `scale`.  A logit or bias of
+    -infinity or NaN masks its expert.  Everything lives on `device_id`."""
+
+    def __init__(self, logits: int, ids: int, weights: int, expert_counts: int, stream_ptr: int, *,
+                 num_tokens: int, num_experts: int, top_k: int, data_type: DataType = DataType.FP32,
+                 score: Score = Score.SOFTMAX, bias: int = 0, num_groups: int = 1,
+                 top_groups: Optional[int] = None, group_score: GroupScore = GroupScore.TOP2,
+                 renormalize: bool = True, scale: float = 1.0, offsets: int = 0, positions: int = 0,
+                 device_id: int = 0):
+        self.stream_ptr = stream_ptr
+        self.c = N.SelectArgsC(logits or None, bias or None, ids or None, weights or None, expert_counts or None,
+                               offsets or None, positions or None, num_tokens, num_experts, top_k, int(data_type),
+                               int(score), num_groups, num_groups if top_groups is None else top_groups,
+                               int(group_score), int(renormalize), scale, device_id)
+
+
+def select(arg: SelectArgs, flash_handle: Optional[ContextHandle] = None) -> None:
+    """Choose experts from logits on `arg.stream_ptr` (fmoe_router_select): softmax or sigmoid scores, a
+    bias for the choice, groups, renormalised or scaled weights.  With `flash_handle` the context's
+    routing table is filled as well, as `router.forward` does, so that `forward(flash_handle, ...)` on
+    the same stream runs on this choice."""
+    N.check(N.lib().fmoe_router_select(flash_handle.context if flash_handle is not None else None, arg.c,
+                                       arg.stream_ptr), "router.select")

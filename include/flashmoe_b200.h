@@ -246,6 +246,156 @@ int fmoe_forward_host_async(fmoe_ctx* ctx, fmoe_router* router, const void* toke
 /* Blocks until every submitted step, its copies included, is done. */
 int fmoe_forward_host_wait(fmoe_ctx* ctx, void* stream);
 
+/* --- routing from logits --------------------------------------------------------------- */
+
+/* No counterpart in the reference, whose gate is softmax, top-k, renormalise.  Routing for models
+ * that score otherwise: sigmoid scores, a balance bias that takes part in the choice only, groups of
+ * experts, unnormalised or scaled weights.  For every token:
+ *   s   = softmax(logits) or sigmoid(logits);   c = s + bias (c = s where bias is null)
+ *   groups: the experts fall into num_groups equal runs; a group's score is the sum of its two
+ *     largest c (FMOE_GROUP_TOP2; of its one expert, where it has one) or its largest
+ *     (FMOE_GROUP_MAX); the top_groups best groups stay
+ *   ids = the top_k largest c of the groups that stay, descending; equal values go to the lower
+ *     index, among groups too
+ *   weights = s[ids], divided by their sum if `renormalize`, times `scale`
+ * The order of the c is that of their exact values: where fp32 cannot tell two apart, they are
+ * compared in 64 bits.  A logit or bias of -infinity or NaN masks its expert: it is chosen only
+ * when nothing else is left, and a masked logit's s is 0; +infinity counts as the largest finite
+ * number.  Where the chosen s sum to 0 the weights are 0. */
+enum { FMOE_SCORE_SOFTMAX = 0, FMOE_SCORE_SIGMOID = 1 };
+enum { FMOE_GROUP_TOP2 = 0, FMOE_GROUP_MAX = 1 };
+typedef struct fmoe_select_args {
+  const void* logits;      /* [num_tokens, num_experts] of data_type */
+  const float* bias;       /* [num_experts] or null */
+  int32_t* ids;            /* [num_tokens, top_k] out */
+  float* weights;          /* [num_tokens, top_k] out */
+  int32_t* expert_counts;  /* [num_experts] out: tokens that chose each expert */
+  int32_t* offsets;        /* [num_experts + 1] out, or null: exclusive sums of expert_counts */
+  int32_t* positions;      /* [num_tokens, top_k] out, or null: the row of every (token, choice) pair
+                              when the pairs are ordered by expert, tokens ascending within one */
+  int32_t num_tokens;      /* >= 0 */
+  int32_t num_experts;     /* 1..1024 */
+  int32_t top_k;           /* 1..32, at most the experts of top_groups groups */
+  int32_t data_type;       /* of the logits: FMOE_DT_BF16, _FP16 or _FP32 */
+  int32_t score;           /* FMOE_SCORE_* */
+  int32_t num_groups;      /* divides num_experts; 1 = no groups; at most 32 */
+  int32_t top_groups;      /* 1..num_groups */
+  int32_t group_score;     /* FMOE_GROUP_* */
+  int32_t renormalize;
+  float scale;
+  int32_t device_id;       /* of every pointer and of `stream`; the caller's current device is kept */
+} fmoe_select_args;
+/* `moe` (may be null): a context of this shape (S, E, k); its routing table and route records are
+ * written too, so that fmoe_forward(moe, ...) on the same stream runs on this choice. */
+int fmoe_router_select(fmoe_ctx* moe, const fmoe_select_args* args, void* stream);
+
+/* --- experts in 8 bits ------------------------------------------------------------------ */
+
+/* No counterpart in the reference.  A matrix in 8 bits is e4m3 codes, row-major, and one fp32 scale
+ * per block: of 1 x 128 values for activations (scale [rows, ceil(cols / 128)]), of 128 x 128 for
+ * weights (scale [matrices, ceil(rows / 128), ceil(cols / 128)]); a code stands for its value times
+ * its block's scale.  Weight layouts are those of fmoe_forward_args.
+ * All calls only launch on `stream`: they allocate nothing, wait for nothing, can be captured, and
+ * keep the caller's current device.  Rows of zero count launch nothing.
+ * "Expert order": rows grouped by expert, `offsets` [num_experts + 1] on the device saying where each
+ * expert's rows begin (what fmoe_router_select writes); rows behind offsets[num_experts] are neither
+ * read for any result nor written.  Offsets and positions outside the rows are ignored. */
+
+/* x [num_matrices, rows, cols] -> codes and scales: scale = amax / 448 of the block, code =
+ * e4m3(448 x / amax), to nearest even; 0 and 0 for a block of zeros.  A block that holds a NaN or an
+ * infinity reads back as NaN.  block_rows: 1 or 128.
+ * With `positions` [rows, copies] (block_rows 1, one matrix) row r is written to output rows
+ * positions[r][0..copies-1] of rows * copies: quantised once, laid out in expert order. */
+typedef struct fmoe_fp8_quantize_args {
+  const void* x;            /* 16-byte aligned */
+  void* q;                  /* out, e4m3; 16-byte aligned */
+  float* scale;             /* out */
+  const int32_t* positions; /* or null */
+  int32_t copies;           /* 1 without positions */
+  int32_t rows;
+  int32_t cols;             /* a multiple of 16 */
+  int32_t num_matrices;
+  int32_t block_rows;
+  int32_t data_type;        /* of x: FMOE_DT_BF16, _FP16 or _FP32 */
+  int32_t device_id;
+} fmoe_fp8_quantize_args;
+int fmoe_fp8_quantize(const fmoe_fp8_quantize_args* args, void* stream);
+
+/* out [m, n] = A [m, k] * W [n, k]^T: the products within a 128-block of k are summed by the tensor
+ * core, the blocks times their scales in fp32, one rounding to data_type at the end.
+ * num_experts 1, offsets null: one product.  Else W [num_experts, n, k], and the rows of A and out
+ * are in expert order. */
+typedef struct fmoe_fp8_matmul_args {
+  const void* a;            /* [m, k] e4m3; 16-byte aligned, as w */
+  const float* a_scale;     /* [m, ceil(k / 128)] */
+  const void* w;            /* [num_experts, n, k] e4m3 */
+  const float* w_scale;     /* [num_experts, ceil(n / 128), ceil(k / 128)] */
+  void* out;                /* [m, n] of data_type, aligned to its type */
+  const int32_t* offsets;   /* [num_experts + 1], or null with one expert */
+  int32_t m;
+  int32_t n;
+  int32_t k;                /* a multiple of 16 */
+  int32_t num_experts;      /* 1..1024 */
+  int32_t data_type;        /* FMOE_DT_BF16, _FP16 or _FP32 */
+  int32_t device_id;
+} fmoe_fp8_matmul_args;
+int fmoe_fp8_matmul(const fmoe_fp8_matmul_args* args, void* stream);
+
+/* The first half of a gated MLP in one kernel: h = act(A up^T) * (A up_v^T) in fp32 (h = act(A up^T)
+ * where up_v is null), left in 8 bits, ready to be the A of the down product. */
+typedef struct fmoe_fp8_gated_args {
+  const void* a;            /* [m, k] e4m3; 16-byte aligned, as up, up_v and q */
+  const float* a_scale;     /* [m, ceil(k / 128)] */
+  const void* up;           /* [num_experts, ffn_size, k] e4m3 */
+  const float* up_scale;    /* [num_experts, ceil(ffn_size / 128), ceil(k / 128)] */
+  const void* up_v;         /* like up, or null */
+  const float* up_v_scale;
+  void* q;                  /* [m, ffn_size] e4m3 out */
+  float* scale;             /* [m, ceil(ffn_size / 128)] out */
+  const int32_t* offsets;   /* as in fmoe_fp8_matmul_args */
+  int32_t m;
+  int32_t ffn_size;         /* a multiple of 16 */
+  int32_t k;                /* a multiple of 16 */
+  int32_t num_experts;
+  int32_t act_type;         /* FMOE_ACT_* */
+  int32_t device_id;
+} fmoe_fp8_gated_args;
+int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* args, void* stream);
+
+/* The expert layer on 8-bit weights: tokens are quantised into expert order, multiplied with up and
+ * up_v, activated and quantised, multiplied with down (rounded to data_type, as the rows that
+ * fmoe_forward returns) and summed per token in fp32 in the order of its choices, one rounding. */
+typedef struct fmoe_fp8_experts_args {
+  const void* tokens;       /* [num_tokens, token_dim] of data_type; 16-byte aligned */
+  const int32_t* offsets;   /* [num_experts + 1], of fmoe_router_select */
+  const int32_t* positions; /* [num_tokens, top_k], of fmoe_router_select */
+  const float* weights;     /* [num_tokens, top_k], of fmoe_router_select */
+  const void* up;           /* [num_experts, ffn_size, token_dim] e4m3, and its scales */
+  const float* up_scale;
+  const void* up_v;         /* like up, or null for a plain MLP */
+  const float* up_v_scale;
+  const void* down;         /* [num_experts, token_dim, ffn_size] e4m3, and its scales */
+  const float* down_scale;
+  void* out;                /* [num_tokens, token_dim] of data_type; 16-byte aligned */
+  void* workspace;          /* 256-byte aligned; calls that share one must be ordered */
+  int64_t workspace_bytes;  /* at least fmoe_fp8_workspace_bytes */
+  int32_t num_tokens;
+  int32_t token_dim;        /* a multiple of 16, as ffn_size */
+  int32_t ffn_size;
+  int32_t num_experts;
+  int32_t top_k;            /* 1..32 */
+  int32_t data_type;        /* FMOE_DT_BF16 or _FP16 */
+  int32_t act_type;         /* FMOE_ACT_* */
+  int32_t device_id;
+} fmoe_fp8_experts_args;
+/* Host arithmetic only; reads the shape fields of `args`. */
+int fmoe_fp8_workspace_bytes(const fmoe_fp8_experts_args* args, int64_t* bytes_out);
+int fmoe_fp8_experts(const fmoe_fp8_experts_args* args, void* stream);
+
+/* The record of the first device-side wait of an 8-bit product on this device that ran out since the
+ * last call (code 0: none); waits for `stream`, then clears the record. */
+int fmoe_fp8_last_status(int32_t device_id, void* stream, fmoe_status* out);
+
 /* --- diagnostics --------------------------------------------------------------------- */
 
 /* Reads the record the last forward left (synchronises `stream` first).  A record with a non-zero
