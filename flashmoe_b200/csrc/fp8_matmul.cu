@@ -7,10 +7,13 @@
 // block's accumulator, scale it and add it to fp32 registers.  The tensor core never sees a scale, so
 // any fp32 scales work, and no sum crosses a block boundary unscaled.
 //
-// One persistent CTA per SM: warp 0 loads tiles (TMA), warp 1 issues the MMAs, warps 2..9 scale and
-// add.  A tile is 128 rows x 256 features (the gated form: 128 features of up and the same 128 of
-// up_v); the two TMEM accumulators of 256 columns let the MMAs of one block run while the other
-// block's sums are read.
+// CTA pairs (clusters of two SMs) work on tiles of 256 rows x 256 features (the gated form: 128 features of
+// up and the same 128 of up_v) with cta_group::2 MMAs: each CTA fetches and accumulates its own 128
+// rows, and half of the weight tile, which the pair's tensor cores share.  A CTA alone would move 48 KB
+// through shared memory per 512 cycles of MMA, in and out again, which is more than shared memory passes;
+// a pair's CTAs move 32 KB.  In a CTA, warp 0 loads tiles (TMA), warp 1 of the leader issues the MMAs,
+// warps 2 and 3 fetch scales, warps 4..11 scale and add.  The two TMEM accumulators of 256 columns
+// let the MMAs of one block run while the other block's sums are read.
 #include <atomic>
 #include <cstdlib>
 #include <mutex>
@@ -23,12 +26,17 @@ namespace {
 
 using namespace fmoe::ptx;
 
-constexpr int kThreads = 320;                  // TMA warp, MMA warp, eight epilogue warps
-constexpr int kEpilogueWarps = 8;
+// TMA warp, MMA warp, two warps that fetch scales, then the epilogue warps: four per 128 rows and
+// kColumnWarps of those side by side along the columns.
+constexpr int kScaleWarp = 2, kScaleWarps = 2, kScaleSlots = 2, kScaleBlocks = 4, kEpilogueWarp = 4;
+constexpr int kColumnWarps = 2, kEpilogueWarps = 4 * kColumnWarps, kThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
+constexpr int kRun = 128 / kColumnWarps;   // columns of one weight block that a warp adds up
+// Registers a thread: 168 at launch (384 threads), then 88 and 208: 4 * 88 + 8 * 208 = 12 * 168.
+constexpr int kLoadRegs = 88, kEpilogueRegs = 208;
 constexpr int kMaxExperts = 1024;
 constexpr uint32_t kBoxBytes = 128 * kBlock;   // 128 rows of one k block: 16 KB
-constexpr int kStages = 4;
-constexpr uint32_t kStageBytes = 3 * kBoxBytes;
+constexpr int kStages = 6;
+constexpr uint32_t kStageBytes = 2 * kBoxBytes;   // 128 rows of each operand
 
 struct Codes {};   // "output type" of the gated form
 
@@ -133,18 +141,25 @@ __device__ __forceinline__ void tmem_wait_16(uint32_t (&r)[16]) {
                : "memory");
 }
 
+// Arrives on a barrier of either CTA of the pair.  What it announces is that TMEM has been read, which tcgen05's
+// own wait and fence order; no memory another CTA looks at, so it needs no release: a release at cluster scope
+// waits for everything the warp has in flight, which halved the rate of the whole kernel.
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&w)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
 
-// 128 features of one row, in order in acc[64] (pairs), to dst; `valid` of them exist.
-template <typename Out>
-__device__ __forceinline__ void store_features(Out* dst, const uint64_t (&acc)[64], int valid, bool wide) {
+// N features of one row, in order in acc (pairs), to dst; `valid` of them exist.
+template <typename Out, int N>
+__device__ __forceinline__ void store_features(Out* dst, const uint64_t* acc, int valid, bool wide) {
   constexpr int kPer = 32 / sizeof(Out);
 #pragma unroll
-  for (int g = 0; g < 128 / kPer; ++g) {
+  for (int g = 0; g < N / kPer; ++g) {
     float f[kPer];
 #pragma unroll
     for (int i = 0; i < kPer / 2; ++i) {
@@ -171,175 +186,263 @@ __device__ __forceinline__ void store_features(Out* dst, const uint64_t (&acc)[6
   }
 }
 
+// A place in the ring of stages, and the parity of the round it is in.
+struct Ring {
+  uint32_t stage = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+
 struct SharedTail {
-  uint64_t full[kStages], empty[kStages];
-  uint64_t acc_full[2], acc_empty[2];
+  uint64_t full[kStages];         // the leader's: both CTAs' copies of the stage have landed
+  uint64_t done[kStages];         // each CTA's: the MMAs of the stage are done: it is free, its sums are in TMEM
+  uint64_t acc_empty[2];          // the leader's: both CTAs have read it
+  uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots];   // each CTA's
+  uint64_t amax_full[4];          // all maxima of a quarter's rows are in
   uint32_t tmem_base;
   uint32_t abort_word;
-  uint32_t amax[2][2][128];   // [tile parity][column half][row]
-  uint64_t amax_full[4];      // both halves' maxima of a quarter's rows are in
+  float scale[kScaleSlots][kScaleBlocks][2][128];   // [block of k][weight block][row]: a's scale times w's
+  uint32_t amax[2][kColumnWarps][128];     // [tile parity]
   TileTable table;
 };
 
 // Rows on the TMEM lanes, features on its columns.
 template <typename Out>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w0,
                const __grid_constant__ CUtensorMap map_w1, const ProductParams p) {
   constexpr bool kGated = std::is_same_v<Out, Codes>;
-  constexpr int kTileM = 128, kTileN = kGated ? 128 : 256;
+  constexpr int kTileM = 256, kTileN = kGated ? 128 : 256;
   extern __shared__ __align__(16) unsigned char s_raw[];
   unsigned char* ring = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);   // swizzle atoms are 1024 bytes
   SharedTail& sh = *reinterpret_cast<SharedTail*>(ring + kStages * kStageBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const WaitCtx wc{&sh.abort_word, p.spin_limit};
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&sh.acc_full[i], 1); mbar_init(&sh.acc_empty[i], kEpilogueWarps); }
-    for (int i = 0; i < 4; ++i) mbar_init(&sh.amax_full[i], 2);
+    for (int i = 0; i < kStages; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.done[i], 1); }
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.acc_empty[i], 2 * kEpilogueWarps);
+    for (int i = 0; i < 4; ++i) mbar_init(&sh.amax_full[i], kColumnWarps);
+    for (int i = 0; i < kScaleSlots; ++i) {
+      mbar_init(&sh.scale_full[i], kScaleWarps);
+      mbar_init(&sh.scale_empty[i], kEpilogueWarps);
+    }
     sh.abort_word = 0;
     mbar_fence_init();
   }
   if (warp == 1) {
-    tmem_alloc(&sh.tmem_base, 512);
-    tmem_relinquish();
+    tmem_alloc_pair(&sh.tmem_base, 512);
+    tmem_relinquish_pair();
   }
   fill_table(sh.table, p, kTileM);
+  cluster_sync_all();   // both CTAs' barriers exist before either is signalled from the other
   tc_fence_after_sync();
   const uint32_t tmem = sh.tmem_base;
   const bool second = !kGated || p.has_v != 0;   // whether the second 128 weight rows exist
 
-  if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t bytes = (second ? 3 : 2) * kBoxBytes;
-      int issued = 0;
-      Tile t;
-      bool ok = true;
-      for (int i = blockIdx.x; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += gridDim.x) {
-        const int w_row = t.expert * p.n + t.n0;   // (host: experts * n fits an int)
-        for (int kb = 0; kb < p.kblocks; ++kb, ++issued) {
-          const int s = issued % kStages;
-          if (!mbar_wait(&sh.empty[s], ((issued / kStages) & 1) ^ 1, wc)) {
-            wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_EMPTY, i);
-            ok = false;
-            break;
+  if (warp < kEpilogueWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+    if (warp == 0) {
+      if (lane == 0) {
+        // a plain MLP has no second weight tile: its follower loads the first one again, into columns nobody reads
+        const CUtensorMap* map_w = rank == 0 ? &map_w0 : &map_w1;
+        Ring at;
+        Tile t;
+        bool ok = true;
+        for (int i = pair; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += pairs) {
+          const int row = t.row0 + static_cast<int>(rank) * 128;
+          const int w_row = t.expert * p.n + t.n0 + (kGated ? 0 : static_cast<int>(rank) * 128);   // (fits: checked by the host)
+          for (int kb = 0; kb < p.kblocks; ++kb) {
+            if (!mbar_wait(&sh.done[at.stage], at.phase ^ 1, wc)) {
+              wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_EMPTY, i);
+              ok = false;
+              break;
+            }
+            unsigned char* stage = ring + at.stage * kStageBytes;
+            if (rank == 0) mbar_expect_tx(&sh.full[at.stage], 2 * kStageBytes);
+            tma_load_2d_pair(stage, &map_a, &sh.full[at.stage], kb * kBlock, row);
+            tma_load_2d_pair(stage + kBoxBytes, map_w, &sh.full[at.stage], kb * kBlock, w_row);
+            at.next();
           }
-          unsigned char* stage = ring + s * kStageBytes;
-          mbar_expect_tx(&sh.full[s], bytes);
-          tma_load_2d(stage, &map_a, &sh.full[s], kb * kBlock, t.row0);
-          tma_load_2d(stage + kBoxBytes, &map_w0, &sh.full[s], kb * kBlock, w_row);
-          if (second) tma_load_2d(stage + 2 * kBoxBytes, &map_w1, &sh.full[s], kb * kBlock, kGated ? w_row : w_row + 128);
+        }
+        // no copy may be in flight when the CTA leaves: the MMAs that free a stage come after its copies
+        const WaitCtx last{nullptr, p.spin_limit};
+        for (int j = 0; j < kStages; ++j) {   // (a stage that was never filled passes at once)
+          mbar_wait(&sh.done[at.stage], at.phase ^ 1, last);
+          at.next();
         }
       }
-      // no copy may be in flight when the CTA leaves (all have been waited for unless a wait ran out)
-      const WaitCtx last{nullptr, p.spin_limit};
-      for (int j = max(0, issued - kStages); j < issued; ++j) mbar_wait(&sh.full[j % kStages], (j / kStages) & 1, last);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = umma_idesc_e4m3(128, second ? 256 : 128);
+    } else if (warp == 1) {
+      if (lane == 0 && rank == 0) {
+        const uint32_t idesc = umma_idesc_e4m3(256, 256);
+        const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
+        Ring at;
+        int b = 0;
+        uint32_t b_phase = 1;
+        Tile t;
+        bool ok = true, ready = false;
+        uint32_t last_stage = 0, last_phase = 1;
+        for (int i = pair; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += pairs) {
+          for (int kb = 0; kb < p.kblocks; ++kb) {
+            if (!ready) {
+              if (!mbar_wait(&sh.acc_empty[b], b_phase, wc)) {
+                wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_EMPTY, i);
+                ok = false;
+                break;
+              }
+              if (!mbar_wait(&sh.full[at.stage], at.phase, wc)) {
+                wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_FULL, i);
+                ok = false;
+                break;
+              }
+            }
+            tc_fence_after_sync();
+            const uint64_t da = desc0 + at.stage * (kStageBytes >> 4), dw = da + (kBoxBytes >> 4);
+  #pragma unroll
+            for (int q = 0; q < 4; ++q)   // 32 bytes of k each
+              umma_f8_pair(tmem + b * 256, da + 2 * q, dw + 2 * q, idesc, q != 0);
+            umma_commit_pair(&sh.done[at.stage], 3);
+            last_stage = at.stage;
+            last_phase = at.phase;
+            at.next();
+            b ^= 1;
+            b_phase ^= b == 0;
+            // look at the next block's barriers while the MMAs run
+            const bool f = mbar_try_wait(&sh.full[at.stage], at.phase), e = mbar_try_wait(&sh.acc_empty[b], b_phase);
+            ready = f && e;
+          }
+        }
+        // no MMA may be running when TMEM is freed
+        const WaitCtx last{nullptr, p.spin_limit};
+        mbar_wait(&sh.done[last_stage], last_phase, last);
+      }
+    } else {
+      // The scales of a block of k go with its accumulator: two rows a lane, loaded four blocks at a time
+      // and four to eight blocks ahead, so that the epilogue never waits for global memory.
+      const int r0 = (warp - kScaleWarp) * 64 + lane;
       int done = 0;
       Tile t;
       bool ok = true;
-      for (int i = blockIdx.x; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += gridDim.x) {
-        for (int kb = 0; kb < p.kblocks; ++kb, ++done) {
-          const int s = done % kStages, b = done & 1;
-          if (!mbar_wait(&sh.acc_empty[b], ((done >> 1) & 1) ^ 1, wc)) {
-            wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_EMPTY, i);
-            ok = false;
-            break;
-          }
-          if (!mbar_wait(&sh.full[s], (done / kStages) & 1, wc)) {
-            wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_FULL, i);
-            ok = false;
-            break;
-          }
-          tc_fence_after_sync();
-          const uint32_t stage = smem_u32(ring + s * kStageBytes);
-          const uint64_t da = umma_desc_sw128(stage), dw = umma_desc_sw128(stage + kBoxBytes);
-#pragma unroll
-          for (int q = 0; q < 4; ++q)   // 32 bytes of k each
-            umma_f8(tmem + b * 256, da + 2 * q, dw + 2 * q, idesc, q != 0);
-          umma_commit(&sh.empty[s]);
-          umma_commit(&sh.acc_full[b]);
+      for (int i = pair; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += pairs) {
+        const float* src[4] = {nullptr, nullptr, nullptr, nullptr};   // this lane's two rows, the two weight blocks
+        for (int j = 0; j < 2; ++j) {
+          const int row = t.row0 + static_cast<int>(rank) * 128 + r0 + 32 * j, nb = t.n0 / kBlock + (kGated ? 0 : j);
+          if (row < t.row_end) src[j] = p.a_scale + static_cast<size_t>(row) * p.kblocks;
+          const float* w = p.w_scale[kGated ? j : 0];
+          if (nb < p.nblocks && w != nullptr) src[2 + j] = w + (static_cast<size_t>(t.expert) * p.nblocks + nb) * p.kblocks;
         }
+        float now[4][4], next[4][4];   // [block][source]
+        auto fetch = [&](int kb, float (&to)[4][4]) {
+  #pragma unroll
+          for (int x = 0; x < 4; ++x)
+  #pragma unroll
+            for (int j = 0; j < 4; ++j) to[x][j] = src[j] != nullptr && kb + x < p.kblocks ? __ldg(src[j] + kb + x) : 0.0f;
+        };
+        fetch(0, next);
+        for (int kb0 = 0; ok && kb0 < p.kblocks; kb0 += 4) {
+  #pragma unroll
+          for (int x = 0; x < 4; ++x)
+  #pragma unroll
+            for (int j = 0; j < 4; ++j) now[x][j] = next[x][j];
+          fetch(kb0 + 4, next);
+          const int slot = done % kScaleSlots;
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.scale_empty[slot], ((done / kScaleSlots) & 1) ^ 1, wc));
+          if (!ok) break;
+  #pragma unroll
+          for (int x = 0; x < 4; ++x)
+  #pragma unroll
+            for (int j = 0; j < 2; ++j)
+  #pragma unroll
+              for (int h = 0; h < 2; ++h) sh.scale[slot][x][h][r0 + 32 * j] = now[x][j] * now[x][2 + h];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.scale_full[slot]);
+          ++done;
+        }
+        if (!ok && lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_EMPTY, i);
       }
-      // no MMA may be running when TMEM is freed
-      const WaitCtx last{nullptr, p.spin_limit};
-      if (done > 0) mbar_wait(&sh.acc_full[(done - 1) & 1], ((done - 1) >> 1) & 1, last);
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;   // TMEM lanes of this warp; its half of the columns
-    const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpilogueRegs));
+    // This warp's 32 rows and 256 / kColumnWarps columns, as two runs of kRun: of both weight blocks in the gated
+    // form (the same features of up and up_v), one after the other in the plain form.
+    const int quarter = warp & 3, column_warp = (warp - kEpilogueWarp) >> 2;
+    constexpr int kSecond = kGated ? 128 : kRun;                        // where the second run begins
+    const int column0 = column_warp * (kGated ? kRun : 2 * kRun);
+    const int block0 = kGated ? 0 : column_warp * 2 / kColumnWarps, block1 = kGated ? 1 : block0;
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + column0;
     const int r = quarter * 32 + lane;
-    int done = 0, parity = 0;
+    const uint32_t acc_empty[2] = {map_to_cta(&sh.acc_empty[0], 0), map_to_cta(&sh.acc_empty[1], 0)};
+    Ring at;
+    int b = 0, groups = 0, parity = 0;
     Tile t;
     bool ok = true;
-    for (int i = blockIdx.x; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += gridDim.x, parity ^= 1) {
-      const int row = t.row0 + r;
+    for (int i = pair; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += pairs, parity ^= 1) {
+      const int row = t.row0 + static_cast<int>(rank) * 128 + r;
       const bool live = row < t.row_end;
-      // scales of this thread's row, and of its first and last 64 columns; two blocks ahead in registers
-      const float* sa = live ? p.a_scale + static_cast<size_t>(row) * p.kblocks : nullptr;
-      const int nb = t.n0 / kBlock + (kGated ? 0 : half);
-      const size_t w_at = (static_cast<size_t>(t.expert) * p.nblocks + nb) * p.kblocks;
-      const float* sw0 = nb < p.nblocks ? p.w_scale[0] + w_at : nullptr;
-      const float* sw1 = kGated ? (second ? p.w_scale[1] + w_at : nullptr) : sw0;
-      auto scale_at = [&](const float* s, int kb) { return s != nullptr && kb < p.kblocks ? __ldg(s + kb) : 0.0f; };
-      float a0 = scale_at(sa, 0), a1 = scale_at(sa, 1);
-      float u0 = scale_at(sw0, 0), u1 = scale_at(sw0, 1);
-      float v0 = kGated ? scale_at(sw1, 0) : 0.0f, v1 = kGated ? scale_at(sw1, 1) : 0.0f;
-      uint64_t acc[64];
+      uint64_t acc[kRun];   // pairs of columns: the first run's, then the second's
 #pragma unroll
-      for (int j = 0; j < 64; ++j) acc[j] = 0;
-      for (int kb = 0; kb < p.kblocks; ++kb, ++done) {
-        const int b = done & 1;
-        const float a = a0, u = u0, v = v0;
-        a0 = a1; u0 = u1; v0 = v1;
-        a1 = scale_at(sa, kb + 2);
-        u1 = scale_at(sw0, kb + 2);
-        if constexpr (kGated) v1 = scale_at(sw1, kb + 2);
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[b], (done >> 1) & 1, wc));
-        if (!ok) {
-          if (lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_FULL, i);
-          break;
-        }
+      for (int j = 0; j < kRun; ++j) acc[j] = 0;
+      constexpr int kChunks = kRun / 8;   // of 16 columns
+      auto column = [&](int c) { return c < kChunks / 2 ? c * 16 : kSecond + (c - kChunks / 2) * 16; };
+#pragma unroll 1
+      for (int kb = 0; kb < p.kblocks; ++kb) {   // (a wait that fails goes on: nothing is stored then)
+        const int slot = groups % kScaleSlots, x = kb % kScaleBlocks;
+        if (x == 0) ok = mbar_wait(&sh.scale_full[slot], (groups / kScaleSlots) & 1, wc) && ok;
+        const float f0 = sh.scale[slot][x][block0][r], f1 = kGated ? sh.scale[slot][x][block1][r] : f0;
+        ok = mbar_wait(&sh.done[at.stage], at.phase, wc) && ok;
+        __syncwarp();
         tc_fence_after_sync();
-        const uint64_t s0 = pack2(a * u, a * u), s1 = kGated ? pack2(a * v, a * v) : s0;
-        // columns of chunk c: this half's 128, or 64 of up and the same 64 of up_v
-        auto column = [&](int c) { return kGated ? (c < 4 ? half * 64 + c * 16 : 128 + half * 64 + (c - 4) * 16) : half * 128 + c * 16; };
-        uint32_t d[2][16];
-        tmem_ld_16(taddr + b * 256 + column(0), d[0]);
+        const uint64_t s0 = pack2(f0, f0), s1 = kGated ? pack2(f1, f1) : s0;
+        uint32_t d[16];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          tmem_wait_16(d[c & 1]);
-          if (c < 7) {
-            tmem_ld_16(taddr + b * 256 + column(c + 1), d[(c + 1) & 1]);
-          } else {
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.acc_empty[b]);
-          }
+        for (int c = 0; c < kChunks - 1; ++c) {
+          tmem_ld_16(taddr + b * 256 + column(c), d);
+          tmem_wait_16(d);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            acc[c * 8 + j] = fma2(pack2(d[c & 1][2 * j], d[c & 1][2 * j + 1]), c < 4 ? s0 : s1, acc[c * 8 + j]);
+          for (int j = 0; j < 8; ++j) acc[c * 8 + j] = fma2(pack2(d[2 * j], d[2 * j + 1]), c < kChunks / 2 ? s0 : s1, acc[c * 8 + j]);
         }
+        tmem_ld_16(taddr + b * 256 + column(kChunks - 1), d);
+        tmem_wait_16(d);
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) arrive_at(acc_empty[b]);
+        if (x == kScaleBlocks - 1 || kb + 1 == p.kblocks) {
+          if (lane == 0) mbar_arrive(&sh.scale_empty[slot]);
+          ++groups;
+        }
+        {
+          constexpr int c = kChunks - 1;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[c * 8 + j] = fma2(pack2(d[2 * j], d[2 * j + 1]), c < kChunks / 2 ? s0 : s1, acc[c * 8 + j]);
+        }
+        at.next();
+        b ^= 1;
       }
-      if (!ok) break;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_FULL, i);
+        break;
+      }
       if constexpr (kGated) {
-        // h = act(up) * up_v of 64 features of this row; the block's maximum with the other half's warp
-        const int col = t.n0 + half * 64;
+        // h = act(up) * up_v of this warp's features; the block's maximum with the row's other warps
+        const int col = t.n0 + column0;
         uint32_t amax = 0;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float2 g = unpack2(acc[j]), w = unpack2(acc[32 + j]);
+        for (int j = 0; j < kRun / 2; ++j) {
+          const float2 g = unpack2(acc[j]), w = unpack2(acc[kRun / 2 + j]);
           float h0 = activate(g.x, p.act), h1 = activate(g.y, p.act);
           if (second) { h0 *= w.x; h1 *= w.y; }
           if (col + 2 * j >= p.n) h0 = h1 = 0.0f;   // (n is even)
           amax = max(amax, max(abs_bits(h0), abs_bits(h1)));
           acc[j] = pack2(h0, h1);
         }
-        sh.amax[parity][half][r] = amax;
+        sh.amax[parity][column_warp][r] = amax;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.amax_full[quarter]);
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.amax_full[quarter], parity, wc));
@@ -347,12 +450,14 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           if (lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TASK, i);
           break;
         }
-        const float top = __uint_as_float(max(sh.amax[parity][0][r], sh.amax[parity][1][r]));
+#pragma unroll
+        for (int j = 0; j < kColumnWarps; ++j) amax = max(amax, sh.amax[parity][j][r]);
+        const float top = __uint_as_float(amax);
         if (live) {
           const Quantizer z(top);
           unsigned char* q = static_cast<unsigned char*>(p.out) + static_cast<size_t>(row) * p.n + col;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
+          for (int g = 0; g < kRun / 16; ++g) {
             if (col + g * 16 < p.n) {   // (n is a multiple of 16)
               uint32_t w[4];
 #pragma unroll
@@ -363,17 +468,18 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
               *reinterpret_cast<uint4*>(q + g * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
-          if (half == 0) p.out_scale[static_cast<size_t>(row) * p.nblocks + t.n0 / kBlock] = block_scale(top);
+          if (column_warp == 0) p.out_scale[static_cast<size_t>(row) * p.nblocks + t.n0 / kBlock] = block_scale(top);
         }
-      } else {
-        const int col = t.n0 + half * 128;
-        if (live && col < p.n)
-          store_features<Out>(static_cast<Out*>(p.out) + static_cast<size_t>(row) * p.n + col, acc, p.n - col, p.wide != 0);
+      } else if (live) {
+        const int col = t.n0 + column0;
+        if (col < p.n)
+          store_features<Out, 2 * kRun>(static_cast<Out*>(p.out) + static_cast<size_t>(row) * p.n + col, acc, p.n - col, p.wide != 0);
       }
     }
   }
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  cluster_sync_all();   // nothing of this CTA's is signalled from the other any more
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
 constexpr size_t kProductSmem = 1024 + kStages * kStageBytes + sizeof(SharedTail);
@@ -446,8 +552,8 @@ ProductParams product_params(int m, int n, int k, int experts, const int32_t* of
 
 int grid_for(const ProductParams& p, int tile_m, int device) {
   const long long most = (static_cast<long long>((p.m + tile_m - 1) / tile_m) + (p.experts > 1 ? p.experts : 0)) * p.tiles_n;
-  const int sms = facts(device).sms;
-  return static_cast<int>(most < sms ? most : sms);
+  const int pairs = facts(device).sms / 2;
+  return 2 * static_cast<int>(most < pairs ? most : pairs);
 }
 
 }  // namespace
@@ -483,7 +589,7 @@ int fmoe_fp8_matmul(const fmoe_fp8_matmul_args* a, void* stream) {
   if (rc == FMOE_OK) rc = make_byte_map(&maps[1], a->w, static_cast<uint64_t>(a->num_experts) * a->n, a->k, 128);
   if (rc != FMOE_OK) return rc;
   maps[2] = maps[1];
-  const int grid = grid_for(p, 128, a->device_id);
+  const int grid = grid_for(p, 256, a->device_id);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->data_type == FMOE_DT_BF16) return launch_product_of<__nv_bfloat16>(p, maps, grid, a->device_id, st);
   if (a->data_type == FMOE_DT_FP16) return launch_product_of<__half>(p, maps, grid, a->device_id, st);
@@ -520,7 +626,7 @@ int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* a, void* stream) {
   if (rc == FMOE_OK) rc = make_byte_map(&maps[1], a->up, w_rows, a->k, 128);
   if (rc == FMOE_OK) rc = make_byte_map(&maps[2], a->up_v != nullptr ? a->up_v : a->up, w_rows, a->k, 128);
   if (rc != FMOE_OK) return rc;
-  return launch_product_of<Codes>(p, maps, grid_for(p, 128, a->device_id), a->device_id, static_cast<cudaStream_t>(stream));
+  return launch_product_of<Codes>(p, maps, grid_for(p, 256, a->device_id), a->device_id, static_cast<cudaStream_t>(stream));
 }
 
 int fmoe_fp8_last_status(int32_t device_id, void* stream, fmoe_status* out) {
