@@ -35,6 +35,17 @@ struct Quantizer {
   }
   __device__ __forceinline__ float scaled(float x) const { return __fdiv_rn(__fmul_rn(x, num), den); }
 };
+// The same for values that carry rounding errors of their own (a product's results): one division per
+// block, then a product per value, at most 2^-23 from the quotient.
+struct FastQuantizer {
+  float pre, inv;   // code = e4m3((pre x) inv)
+  __device__ __forceinline__ explicit FastQuantizer(float amax) {
+    const bool tiny = amax < 0x1p-100f;                // 448 / amax must stay finite, and not underflow
+    pre = tiny ? 0x1p+80f : 1.0f;
+    inv = amax > 0.0f ? __fdiv_rn(kE4m3Max, amax * pre) : (amax == 0.0f ? 0.0f : amax);
+  }
+  __device__ __forceinline__ float scaled(float x) const { return (x * pre) * inv; }
+};
 __device__ __forceinline__ float block_scale(float amax) { return __fdiv_rn(amax, kE4m3Max); }
 // Two values to two codes (lo in the low byte), round to nearest even.
 __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
@@ -94,9 +105,22 @@ __device__ __forceinline__ uint4 pack16(const float (&f)[16 / sizeof(T)]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// x sigmoid(x) within 2^-21 of its value: exp(-x) = 2^n 2^f with f = -x log2(e) - n kept to fp32 precision
+// (log2(e) in two parts), so that only the hardware's exponential (2^-22), the sum and the reciprocal
+// (2^-23) round.
+__device__ __forceinline__ float silu(float x) {
+  const float y = fminf(fmaxf(-x, -87.0f), 87.0f);   // 2^n stays a normal number
+  const float n = rintf(y * 1.44269502e+00f);
+  const float f = fmaf(y, 1.92596303e-08f, fmaf(y, 1.44269502e+00f, -n));
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(f));
+  e = fmaf(e, __int_as_float((static_cast<int>(n) + 127) << 23), 1.0f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e));
+  return x < -87.0f ? 0.0f : x * r;   // (below -87 the value is above -2^-118)
+}
 __device__ __forceinline__ float activate(float x, int act) {
   switch (act) {
-    case FMOE_ACT_SILU: return x / (1.0f + expf(-x));
+    case FMOE_ACT_SILU: return silu(x);
     case FMOE_ACT_GELU: return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
     case FMOE_ACT_RELU: return fmaxf(x, 0.0f);
     default: return x;
@@ -117,6 +141,16 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, u
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// One CTA: D[tmem, 128 rows] (+)= A[smem, 128 rows] * B[smem, N rows]^T over 32 bytes of K.
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
@@ -161,6 +195,5 @@ struct OnDevice {
 };
 inline bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 inline int element_bytes(int data_type) { return data_type == FMOE_DT_FP32 ? 4 : 2; }
-int sm_count(int device);   // cached per device
 
 }  // namespace fmoe::fp8

@@ -454,7 +454,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         for (int j = 0; j < kColumnWarps; ++j) amax = max(amax, sh.amax[parity][j][r]);
         const float top = __uint_as_float(amax);
         if (live) {
-          const Quantizer z(top);
+          const FastQuantizer z(top);
           unsigned char* q = static_cast<unsigned char*>(p.out) + static_cast<size_t>(row) * p.n + col;
 #pragma unroll
           for (int g = 0; g < kRun / 16; ++g) {
@@ -482,6 +482,382 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
+// ---- few rows -----------------------------------------------------------------------------------------
+//
+// Where an expert (or the whole product) has few rows, reading the weights is what there is to do, and the
+// roles turn round: 128 features on the TMEM lanes, kRows rows on its columns, one CTA a tile, and as many
+// bytes of weights in flight as shared memory holds.  The gated form multiplies the tiles of up and up_v with
+// the same rows, into accumulators side by side.  Where the tiles alone do not fill the GPU, the CTAs of a
+// cluster share a tile: each takes a run of the blocks of k, leaves its sums in its shared memory, and adds
+// up, in rank order, the sums of all for its share of the rows.
+
+constexpr int kNarrowThreads = 384;   // TMA, MMA, scale warp, one idle; eight epilogue warps
+constexpr int kMaxSplits = 8;
+constexpr uint32_t kNarrowSmem = 208 * 1024;   // for the ring of stages
+
+template <bool kGated, int kRows>
+struct Narrow {
+  static constexpr int kWeights = kGated ? 2 : 1;
+  static constexpr uint32_t kRowBytes = kRows * kBlock;
+  static constexpr uint32_t kStageBytes = kWeights * kBoxBytes + kRowBytes;
+  static constexpr int kPart = kRows / 2;                       // columns of a weight that one warp adds up
+  static constexpr uint32_t kReduceBytes = kRows <= 32 ? kWeights * kRows * 128 * sizeof(float) : 0;   // splits only
+  static constexpr int kStages = (kNarrowSmem - kReduceBytes) / kStageBytes;
+  static constexpr uint32_t kAccColumns = kWeights * kRows;
+  static constexpr int kAccs = kAccColumns <= 128 ? 4 : 512 / kAccColumns;   // accumulators in flight
+  static constexpr uint32_t kTmemColumns = kAccs * kAccColumns;
+  struct Tail {
+    uint64_t full[kStages], done[kStages];
+    uint64_t acc_empty[kAccs];
+    uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots];
+    uint64_t amax_full[2];
+    uint64_t sums_full, sums_empty;        // the cluster's sums of a tile are there; have been read by all
+    uint32_t tmem_base;
+    uint32_t abort_word;
+    alignas(16) float scale[kScaleSlots][kScaleBlocks][kWeights][kRows];   // (read four at a time)
+    uint32_t amax[2][8][kPart];
+    TileTable table;
+  };
+  static constexpr size_t kSmem = 1024 + kStages * kStageBytes + kReduceBytes + sizeof(Tail);
+};
+
+template <int N>
+__device__ __forceinline__ void tmem_ld_n(uint32_t taddr, uint32_t (&r)[N]) {
+  if constexpr (N == 16) {
+    tmem_ld_16(taddr, r);
+  } else {
+    static_assert(N == 8);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+  }
+}
+template <int N>
+__device__ __forceinline__ void tmem_wait_n(uint32_t (&r)[N]) {
+  if constexpr (N == 16) {
+    tmem_wait_16(r);
+  } else {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+                 :
+                 : "memory");
+  }
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <typename Out, int kRows>
+__global__ void __launch_bounds__(kNarrowThreads, 1)
+product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w0,
+                      const __grid_constant__ CUtensorMap map_w1, const ProductParams p) {
+  constexpr bool kGated = std::is_same_v<Out, Codes>;
+  using N = Narrow<kGated, kRows>;
+  constexpr int kStages = N::kStages, kPart = N::kPart;
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  unsigned char* ring = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);
+  float* sums = reinterpret_cast<float*>(ring + kStages * N::kStageBytes);   // [weight][row][feature], splits only
+  auto& sh = *reinterpret_cast<typename N::Tail*>(ring + kStages * N::kStageBytes + N::kReduceBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_ctarank());
+  const int first_tile = blockIdx.x / splits, tile_step = gridDim.x / splits;
+  const int kb0 = p.kblocks * rank / splits, kb1 = p.kblocks * (rank + 1) / splits;   // this CTA's blocks of k
+  const WaitCtx wc{&sh.abort_word, p.spin_limit};
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.done[i], 1); }
+    for (int i = 0; i < N::kAccs; ++i) mbar_init(&sh.acc_empty[i], kEpilogueWarps);
+    for (int i = 0; i < kScaleSlots; ++i) { mbar_init(&sh.scale_full[i], 1); mbar_init(&sh.scale_empty[i], kEpilogueWarps); }
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.amax_full[i], 4);
+    mbar_init(&sh.sums_full, kEpilogueWarps * splits);
+    mbar_init(&sh.sums_empty, kEpilogueWarps * splits);
+    sh.abort_word = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sh.tmem_base, N::kTmemColumns);
+    tmem_relinquish();
+  }
+  fill_table(sh.table, p, kRows);
+  if (splits > 1) cluster_sync_all();   // the others' barriers exist before any is signalled
+  tc_fence_after_sync();
+  const uint32_t tmem = sh.tmem_base;
+  const bool second = kGated && p.has_v != 0;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t bytes = N::kRowBytes + (second ? 2 : 1) * kBoxBytes;
+      uint32_t stage = 0, phase = 1;
+      Tile t;
+      bool ok = true;
+      for (int i = first_tile; ok && find_tile(sh.table, p.experts, i, kRows, kBlock, t); i += tile_step) {
+        const int w_row = t.expert * p.n + t.n0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&sh.done[stage], phase, wc)) {
+            wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_EMPTY, i);
+            ok = false;
+            break;
+          }
+          unsigned char* to = ring + stage * N::kStageBytes;
+          mbar_expect_tx(&sh.full[stage], bytes);
+          tma_load_2d(to, &map_w0, &sh.full[stage], kb * kBlock, w_row);
+          if (second) tma_load_2d(to + kBoxBytes, &map_w1, &sh.full[stage], kb * kBlock, w_row);
+          tma_load_2d(to + N::kWeights * kBoxBytes, &map_a, &sh.full[stage], kb * kBlock, t.row0);
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+        }
+      }
+      // no copy may be in flight when the CTA leaves: the MMAs that free a stage come after its copies
+      const WaitCtx last{nullptr, p.spin_limit};
+      for (int j = 0; j < kStages; ++j) {   // (a stage that was never filled passes at once)
+        mbar_wait(&sh.done[stage], phase, last);
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_e4m3(128, kRows);
+      const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
+      uint32_t stage = 0, phase = 0, b = 0, b_phase = 1, last_stage = 0, last_phase = 1;
+      Tile t;
+      bool ok = true;
+      for (int i = first_tile; ok && find_tile(sh.table, p.experts, i, kRows, kBlock, t); i += tile_step) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&sh.acc_empty[b], b_phase, wc)) {
+            wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_EMPTY, i);
+            ok = false;
+            break;
+          }
+          if (!mbar_wait(&sh.full[stage], phase, wc)) {
+            wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_FULL, i);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint64_t dw = desc0 + stage * (N::kStageBytes >> 4), da = dw + (N::kWeights * kBoxBytes >> 4);
+          const uint32_t acc = tmem + b * N::kAccColumns;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {   // 32 bytes of k each
+            umma_f8(acc, dw + 2 * q, da + 2 * q, idesc, q != 0);
+            if (second) umma_f8(acc + kRows, dw + (kBoxBytes >> 4) + 2 * q, da + 2 * q, idesc, q != 0);
+          }
+          umma_commit(&sh.done[stage]);
+          last_stage = stage;
+          last_phase = phase;
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+          if (++b == N::kAccs) { b = 0; b_phase ^= 1; }
+        }
+      }
+      const WaitCtx last{nullptr, p.spin_limit};
+      mbar_wait(&sh.done[last_stage], last_phase, last);   // no MMA may be running when TMEM is freed
+    }
+  } else if (warp == kScaleWarp) {
+    // each lane up to four rows, four blocks of k at a time, four to eight blocks ahead
+    constexpr int kLaneRows = kRows < 32 ? 1 : kRows / 32;
+    int groups = 0;
+    Tile t;
+    bool ok = true;
+    for (int i = first_tile; ok && find_tile(sh.table, p.experts, i, kRows, kBlock, t); i += tile_step) {
+      const size_t w_at = (static_cast<size_t>(t.expert) * p.nblocks + t.n0 / kBlock) * p.kblocks;
+      const float* w[2] = {p.w_scale[0] + w_at, second ? p.w_scale[1] + w_at : p.w_scale[0] + w_at};
+      float a_next[kLaneRows][4], w_next[2][4];
+      auto fetch = [&](int kb) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const bool in = kb + x < kb1;
+#pragma unroll
+          for (int j = 0; j < kLaneRows; ++j) {
+            const int row = t.row0 + lane + 32 * j;
+            a_next[j][x] = in && lane + 32 * j < kRows && row < t.row_end
+                               ? __ldg(p.a_scale + static_cast<size_t>(row) * p.kblocks + kb + x) : 0.0f;
+          }
+#pragma unroll
+          for (int h = 0; h < N::kWeights; ++h) w_next[h][x] = in ? __ldg(w[h] + kb + x) : 0.0f;
+        }
+      };
+      fetch(kb0);
+      for (int kb = kb0; kb < kb1; kb += 4, ++groups) {
+        float v[N::kWeights][kLaneRows][4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int j = 0; j < kLaneRows; ++j)
+#pragma unroll
+            for (int h = 0; h < N::kWeights; ++h) v[h][j][x] = a_next[j][x] * w_next[h][x];
+        if (kb + 4 < kb1) fetch(kb + 4);
+        const int slot = groups % kScaleSlots;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.scale_empty[slot], ((groups / kScaleSlots) & 1) ^ 1, wc));
+        if (!ok) break;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int j = 0; j < kLaneRows; ++j)
+#pragma unroll
+            for (int h = 0; h < N::kWeights; ++h)
+              if (lane + 32 * j < kRows) sh.scale[slot][x][h][lane + 32 * j] = v[h][j][x];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.scale_full[slot]);
+      }
+      if (!ok && lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_EMPTY, i);
+    }
+  } else if (warp >= kEpilogueWarp) {
+    // 32 features (a lane each) and half of the rows
+    const int quarter = warp & 3, half = (warp - kEpilogueWarp) >> 2;
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * kPart;
+    constexpr int kChunk = kPart < 16 ? kPart : 16;
+    uint32_t stage = 0, phase = 0, b = 0;
+    int groups = 0, parity = 0;
+    Tile t;
+    bool ok = true;
+    for (int i = first_tile; ok && find_tile(sh.table, p.experts, i, kRows, kBlock, t); i += tile_step, parity ^= 1) {
+      const int feature = t.n0 + quarter * 32 + lane;
+      uint64_t acc[N::kWeights][kPart / 2];   // pairs of rows
+#pragma unroll
+      for (int h = 0; h < N::kWeights; ++h)
+#pragma unroll
+        for (int j = 0; j < kPart / 2; ++j) acc[h][j] = 0;
+#pragma unroll 1
+      for (int kb = kb0; kb < kb1; ++kb) {   // (a wait that fails goes on: nothing is stored then)
+        const int slot = groups % kScaleSlots, x = (kb - kb0) % kScaleBlocks;
+        if (x == 0) ok = mbar_wait(&sh.scale_full[slot], (groups / kScaleSlots) & 1, wc) && ok;
+        ok = mbar_wait(&sh.done[stage], phase, wc) && ok;
+        __syncwarp();
+        tc_fence_after_sync();
+#pragma unroll
+        for (int h = 0; h < N::kWeights; ++h) {
+#pragma unroll
+          for (int c = 0; c < kPart / kChunk; ++c) {
+            uint32_t d[kChunk];
+            tmem_ld_n<kChunk>(taddr + b * N::kAccColumns + h * kRows + c * kChunk, d);
+            const ulonglong2* s = reinterpret_cast<const ulonglong2*>(&sh.scale[slot][x][h][half * kPart + c * kChunk]);
+            tmem_wait_n<kChunk>(d);
+#pragma unroll
+            for (int j = 0; j < kChunk / 4; ++j) {
+              const ulonglong2 f = s[j];   // the scales of four rows
+              uint64_t* to = &acc[h][c * (kChunk / 2) + 2 * j];
+              to[0] = fma2(pack2(d[4 * j], d[4 * j + 1]), f.x, to[0]);
+              to[1] = fma2(pack2(d[4 * j + 2], d[4 * j + 3]), f.y, to[1]);
+            }
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.acc_empty[b]);
+        if (x == kScaleBlocks - 1 || kb + 1 == kb1) {
+          if (lane == 0) mbar_arrive(&sh.scale_empty[slot]);
+          ++groups;
+        }
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+        if (++b == N::kAccs) b = 0;
+      }
+      // the rows this warp finishes: [from, from + count) of its half, sums in value(h, j)
+      int from = 0, count = kPart;
+      if (splits > 1) {
+        // leave the sums where the cluster can read them, then add up this CTA's share of the rows
+        ok = mbar_wait_cluster(&sh.sums_empty, parity ^ 1, wc) && ok;   // the last tile's have been read
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < N::kWeights; ++h)
+#pragma unroll
+          for (int j = 0; j < kPart / 2; ++j) {
+            const float2 v = unpack2(acc[h][j]);
+            float* to = sums + (h * kRows + half * kPart + 2 * j) * 128 + quarter * 32 + lane;
+            to[0] = v.x;
+            to[128] = v.y;
+          }
+        __syncwarp();
+        if (lane < splits) mbar_arrive_cluster(map_to_cta(&sh.sums_full, lane));
+        ok = __all_sync(0xffffffffu, mbar_wait_cluster(&sh.sums_full, parity, wc) && ok);
+        count = kPart / splits;              // (kPart is a multiple of splits)
+        from = rank * count;
+#pragma unroll
+        for (int h = 0; h < N::kWeights; ++h)
+#pragma unroll
+          for (int j = 0; j < kPart / 2; ++j) acc[h][j] = 0;
+        if (ok) {
+          for (int q = 0; q < splits; ++q) {
+#pragma unroll
+            for (int h = 0; h < N::kWeights; ++h) {
+              const uint32_t at = map_to_cta(sums + (h * kRows + half * kPart + from) * 128 + quarter * 32 + lane, q);
+#pragma unroll
+              for (int j = 0; j < kPart / 2; ++j) {
+                if (2 * j < count) {
+                  const float2 v = unpack2(acc[h][j]);
+                  acc[h][j] = pack2(v.x + ld_cluster(at + 2 * j * 128 * sizeof(float)),
+                                    2 * j + 1 < count ? v.y + ld_cluster(at + (2 * j + 1) * 128 * sizeof(float)) : 0.0f);
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane < splits) mbar_arrive_cluster(map_to_cta(&sh.sums_empty, lane));
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_FULL, i);
+        break;
+      }
+      const int row0 = t.row0 + half * kPart + from;
+      if constexpr (kGated) {
+        uint32_t* amax = sh.amax[parity][half * 4 + quarter];
+#pragma unroll
+        for (int j = 0; j < kPart / 2; ++j) {
+          const float2 g = unpack2(acc[0][j]), u = unpack2(acc[1][j]);
+          float h0 = activate(g.x, p.act), h1 = activate(g.y, p.act);
+          if (second) { h0 *= u.x; h1 *= u.y; }
+          if (feature >= p.n) h0 = h1 = 0.0f;
+          acc[0][j] = pack2(h0, h1);
+          const uint32_t m0 = __reduce_max_sync(0xffffffffu, abs_bits(h0)), m1 = __reduce_max_sync(0xffffffffu, abs_bits(h1));
+          if (lane == 0) {
+            amax[2 * j] = m0;
+            amax[2 * j + 1] = m1;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.amax_full[half]);
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.amax_full[half], parity, wc));
+        if (!ok) {
+          if (lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TASK, i);
+          break;
+        }
+#pragma unroll
+        for (int j = 0; j < kPart; ++j) {
+          const int row = row0 + j;
+          if (j < count && row < t.row_end) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) m = max(m, sh.amax[parity][half * 4 + q][j]);
+            const float top = __uint_as_float(m);
+            const float2 v = unpack2(acc[0][j / 2]);
+            const float h = FastQuantizer(top).scaled(j & 1 ? v.y : v.x);
+            if (feature < p.n)
+              static_cast<unsigned char*>(p.out)[static_cast<size_t>(row) * p.n + feature] = static_cast<unsigned char>(to_e4m3x2(h, 0.0f));
+            if (quarter == 0 && lane == 0) p.out_scale[static_cast<size_t>(row) * p.nblocks + t.n0 / kBlock] = block_scale(top);
+          }
+        }
+      } else if (feature < p.n) {
+        Out* to = static_cast<Out*>(p.out) + static_cast<size_t>(row0) * p.n + feature;
+#pragma unroll
+        for (int j = 0; j < kPart; ++j) {
+          const float2 v = unpack2(acc[0][j / 2]);
+          if (j < count && row0 + j < t.row_end) to[static_cast<size_t>(j) * p.n] = from_float<Out>(j & 1 ? v.y : v.x);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (splits > 1) cluster_sync_all();   // the others read this CTA's sums and signal its barriers
+  if (warp == 1) tmem_dealloc(tmem, N::kTmemColumns);
+}
+
 constexpr size_t kProductSmem = 1024 + kStages * kStageBytes + sizeof(SharedTail);
 static_assert(kProductSmem <= 227 * 1024, "shared memory of one CTA");
 
@@ -502,20 +878,98 @@ const DeviceFacts& facts(int device) {
   return all[device];
 }
 
-template <typename Out>
-int launch_product_of(const ProductParams& p, const CUtensorMap (&maps)[3], int grid, int device, cudaStream_t stream) {
-  static std::atomic<unsigned long long> prepared{0};   // devices whose shared-memory limit was raised
-  if (!(prepared.load(std::memory_order_acquire) >> device & 1)) {
-    const cudaError_t e = cudaFuncSetAttribute(product_kernel<Out>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(kProductSmem));
+// Launches a kernel in clusters of `cluster` CTAs (0: its own compile-time shape).
+template <typename Kernel>
+int launch_kernel(Kernel kernel, std::atomic<unsigned long long>& prepared, size_t smem, int threads, int grid, int cluster,
+                  const CUtensorMap (&maps)[3], const ProductParams& p, int device, cudaStream_t stream) {
+  cudaError_t e = cudaSuccess;
+  if (!(prepared.load(std::memory_order_acquire) >> device & 1)) {   // once a device: raise the shared-memory limit
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("8-bit product: ") + cudaGetErrorString(e));
     prepared.fetch_or(1ull << device, std::memory_order_release);
   }
-  product_kernel<Out><<<grid, kThreads, kProductSmem, stream>>>(maps[0], maps[1], maps[2], p);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], p);
   ++g_launches;
-  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("8-bit product launch: ") + cudaGetErrorString(e));
   return FMOE_OK;
+}
+
+template <typename Out>
+int launch_wide(const ProductParams& p, const CUtensorMap (&maps)[3], int grid, int device, cudaStream_t stream) {
+  static std::atomic<unsigned long long> prepared{0};
+  return launch_kernel(product_kernel<Out>, prepared, kProductSmem, kThreads, grid, 0, maps, p, device, stream);
+}
+template <typename Out, int kRows>
+int launch_narrow(const ProductParams& p, const CUtensorMap (&maps)[3], int grid, int splits, int device, cudaStream_t stream) {
+  using N = Narrow<std::is_same_v<Out, Codes>, kRows>;
+  static_assert(N::kSmem <= 227 * 1024, "shared memory of one CTA");
+  static std::atomic<unsigned long long> prepared{0};
+  return launch_kernel(product_narrow_kernel<Out, kRows>, prepared, N::kSmem, kNarrowThreads, grid, splits, maps, p, device, stream);
+}
+
+// Which kernel a product takes, and its launch shape.
+struct Shape {
+  int rows;     // rows a tile has: 256 (pairs), or 16, 32, 64, 128 (few rows)
+  int splits;   // CTAs that share a tile (few rows only)
+  int grid;
+};
+
+Shape shape_for(int m, int features, int kblocks, int experts, int features_wide, int sms) {
+  Shape s{256, 1, 0};
+  const int hit = experts > 1 ? (m < experts ? m : experts) : 1;
+  const double mean = static_cast<double>(m) / hit;
+  if (mean <= 12 || (experts == 1 && m <= 16)) s.rows = 16;
+  else if (mean <= 24 || (experts == 1 && m <= 32)) s.rows = 32;
+  else if (mean <= 48 || (experts == 1 && m <= 64)) s.rows = 64;
+  else if (mean <= 128) s.rows = 128;
+  const int tile_n = s.rows == 256 ? features_wide : kBlock;
+  const long long tiles_n = (features + tile_n - 1) / tile_n;
+  // at most this many tiles (how the rows spread over the experts is known on the device only)
+  const long long tiles = (m / s.rows + hit) * tiles_n;
+  if (s.rows == 256) {
+    const long long pairs = sms / 2;
+    s.grid = 2 * static_cast<int>(tiles < pairs ? tiles : pairs);
+    return s;
+  }
+  while (s.rows <= 32 && s.splits < kMaxSplits && 2 * s.splits <= s.rows / 2 && tiles * s.splits * 2 <= sms &&
+         kblocks >= 8 * s.splits)
+    s.splits *= 2;
+  const long long most = sms / s.splits;
+  s.grid = s.splits * static_cast<int>(tiles < most ? tiles : most);
+  return s;
+}
+
+template <typename Out>
+int launch_product(ProductParams p, const void* a, const void* w0, const void* w1, int device, cudaStream_t stream) {
+  constexpr int kWideN = std::is_same_v<Out, Codes> ? 128 : 256;
+  const Shape s = shape_for(p.m, p.n, p.kblocks, p.experts, kWideN, facts(device).sms);
+  const int tile_n = s.rows == 256 ? kWideN : kBlock;
+  p.tiles_n = (p.n + tile_n - 1) / tile_n;
+  CUtensorMap maps[3];
+  const uint64_t w_rows = static_cast<uint64_t>(p.experts) * p.n;
+  int rc = make_byte_map(&maps[0], a, p.m, p.k, s.rows == 256 ? 128 : s.rows);
+  if (rc == FMOE_OK) rc = make_byte_map(&maps[1], w0, w_rows, p.k, 128);
+  if (rc == FMOE_OK && w1 != w0) rc = make_byte_map(&maps[2], w1, w_rows, p.k, 128);
+  if (rc != FMOE_OK) return rc;
+  if (w1 == w0) maps[2] = maps[1];
+  switch (s.rows) {
+    case 16: return launch_narrow<Out, 16>(p, maps, s.grid, s.splits, device, stream);
+    case 32: return launch_narrow<Out, 32>(p, maps, s.grid, s.splits, device, stream);
+    case 64: return launch_narrow<Out, 64>(p, maps, s.grid, s.splits, device, stream);
+    case 128: return launch_narrow<Out, 128>(p, maps, s.grid, s.splits, device, stream);
+    default: return launch_wide<Out>(p, maps, s.grid, device, stream);
+  }
 }
 
 // The checks that both products share.
@@ -539,26 +993,17 @@ int check_product(const void* a, const float* a_scale, const void* w, const floa
   return FMOE_OK;
 }
 
-ProductParams product_params(int m, int n, int k, int experts, const int32_t* offsets, int tile_n, int device) {
+ProductParams product_params(int m, int n, int k, int experts, const int32_t* offsets, int device) {
   ProductParams p{};
   p.m = m; p.n = n; p.k = k;
   p.kblocks = blocks_of(k); p.nblocks = blocks_of(n);
   p.experts = experts;
   p.offsets = offsets;
-  p.tiles_n = (n + tile_n - 1) / tile_n;
   p.spin_limit = facts(device).spin_limit;
   return p;
 }
 
-int grid_for(const ProductParams& p, int tile_m, int device) {
-  const long long most = (static_cast<long long>((p.m + tile_m - 1) / tile_m) + (p.experts > 1 ? p.experts : 0)) * p.tiles_n;
-  const int pairs = facts(device).sms / 2;
-  return 2 * static_cast<int>(most < pairs ? most : pairs);
-}
-
 }  // namespace
-
-int sm_count(int device) { return facts(device).sms; }
 
 }  // namespace fmoe::fp8
 
@@ -579,21 +1024,15 @@ int fmoe_fp8_matmul(const fmoe_fp8_matmul_args* a, void* stream) {
   if (misaligned(a->out, eb)) return set_error(FMOE_ERR_INVALID_ARG, "out must be aligned to its type");
   OnDevice on(a->device_id);
   if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));
-  ProductParams p = product_params(a->m, a->n, a->k, a->num_experts, a->offsets, 256, a->device_id);
+  ProductParams p = product_params(a->m, a->n, a->k, a->num_experts, a->offsets, a->device_id);
   p.a_scale = a->a_scale;
   p.w_scale[0] = a->w_scale;
   p.out = a->out;
   p.wide = !misaligned(a->out, 32) && (static_cast<size_t>(a->n) * eb) % 32 == 0;
-  CUtensorMap maps[3];
-  rc = make_byte_map(&maps[0], a->a, a->m, a->k, 128);
-  if (rc == FMOE_OK) rc = make_byte_map(&maps[1], a->w, static_cast<uint64_t>(a->num_experts) * a->n, a->k, 128);
-  if (rc != FMOE_OK) return rc;
-  maps[2] = maps[1];
-  const int grid = grid_for(p, 256, a->device_id);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->data_type == FMOE_DT_BF16) return launch_product_of<__nv_bfloat16>(p, maps, grid, a->device_id, st);
-  if (a->data_type == FMOE_DT_FP16) return launch_product_of<__half>(p, maps, grid, a->device_id, st);
-  return launch_product_of<float>(p, maps, grid, a->device_id, st);
+  if (a->data_type == FMOE_DT_BF16) return launch_product<__nv_bfloat16>(p, a->a, a->w, a->w, a->device_id, st);
+  if (a->data_type == FMOE_DT_FP16) return launch_product<__half>(p, a->a, a->w, a->w, a->device_id, st);
+  return launch_product<float>(p, a->a, a->w, a->w, a->device_id, st);
 }
 
 int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* a, void* stream) {
@@ -612,7 +1051,7 @@ int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* a, void* stream) {
   if (a->up_v != nullptr && a->up_v_scale == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "up_v needs its scales");
   OnDevice on(a->device_id);
   if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));
-  ProductParams p = product_params(a->m, a->ffn_size, a->k, a->num_experts, a->offsets, 128, a->device_id);
+  ProductParams p = product_params(a->m, a->ffn_size, a->k, a->num_experts, a->offsets, a->device_id);
   p.a_scale = a->a_scale;
   p.w_scale[0] = a->up_scale;
   p.w_scale[1] = a->up_v_scale;
@@ -620,13 +1059,7 @@ int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* a, void* stream) {
   p.out_scale = a->scale;
   p.act = a->act_type;
   p.has_v = a->up_v != nullptr;
-  CUtensorMap maps[3];
-  const uint64_t w_rows = static_cast<uint64_t>(a->num_experts) * a->ffn_size;
-  rc = make_byte_map(&maps[0], a->a, a->m, a->k, 128);
-  if (rc == FMOE_OK) rc = make_byte_map(&maps[1], a->up, w_rows, a->k, 128);
-  if (rc == FMOE_OK) rc = make_byte_map(&maps[2], a->up_v != nullptr ? a->up_v : a->up, w_rows, a->k, 128);
-  if (rc != FMOE_OK) return rc;
-  return launch_product_of<Codes>(p, maps, grid_for(p, 256, a->device_id), a->device_id, static_cast<cudaStream_t>(stream));
+  return launch_product<Codes>(p, a->a, a->up, a->up_v != nullptr ? a->up_v : a->up, a->device_id, static_cast<cudaStream_t>(stream));
 }
 
 int fmoe_fp8_last_status(int32_t device_id, void* stream, fmoe_status* out) {
