@@ -60,45 +60,51 @@ struct Tile {
   int expert, row0, row_end, n0;
 };
 
-// Which rows each expert has and how many tiles come before it; filled once per CTA.
+// How many tiles come before each expert's; filled once per CTA.
 struct TileTable {
-  int begin[kMaxExperts];
-  int rows[kMaxExperts];
   int first[kMaxExperts + 1];
 };
 
-__device__ __forceinline__ bool find_tile(const TileTable& t, int experts, int tile, int tile_m, int tile_n, Tile& out) {
-  if (tile >= t.first[experts]) return false;
-  int lo = 0, hi = experts - 1;
+// An expert's rows: whatever the array of offsets holds, they stay inside [0, m).
+__device__ __forceinline__ void expert_rows(const ProductParams& p, int e, int& begin, int& end) {
+  begin = 0;
+  end = p.m;
+  if (p.offsets != nullptr) {
+    begin = min(max(__ldg(p.offsets + e), 0), p.m);
+    end = min(max(__ldg(p.offsets + e + 1), begin), p.m);
+  }
+}
+
+__device__ __forceinline__ bool find_tile(const TileTable& t, const ProductParams& p, int tile, int tile_m, int tile_n, Tile& out) {
+  if (tile >= t.first[p.experts]) return false;
+  int lo = 0, hi = p.experts - 1;
   while (lo < hi) {                      // the last expert that begins at or before this tile
     const int mid = (lo + hi + 1) >> 1;
     if (t.first[mid] <= tile) lo = mid; else hi = mid - 1;
   }
-  const int m_tiles = (t.rows[lo] + tile_m - 1) / tile_m, i = tile - t.first[lo];
+  int begin, end;
+  expert_rows(p, lo, begin, end);
+  const int m_tiles = (end - begin + tile_m - 1) / tile_m, i = tile - t.first[lo];
   out.expert = lo;                       // rows first: neighbouring CTAs share a weight tile
-  out.row0 = t.begin[lo] + (i % m_tiles) * tile_m;
-  out.row_end = t.begin[lo] + t.rows[lo];
+  out.row0 = begin + (i % m_tiles) * tile_m;
+  out.row_end = end;
   out.n0 = (i / m_tiles) * tile_n;
   return true;
 }
 
-// Called by every thread; `experts` entries, tile counts summed by warp 0.
+// Called by every thread; the tile counts are summed by warp 0.
 __device__ void fill_table(TileTable& t, const ProductParams& p, int tile_m) {
   for (int e = threadIdx.x; e < p.experts; e += blockDim.x) {
-    int begin = 0, end = p.m;
-    if (p.offsets != nullptr) {          // whatever the array holds, rows stay inside [0, m)
-      begin = min(max(__ldg(p.offsets + e), 0), p.m);
-      end = min(max(__ldg(p.offsets + e + 1), begin), p.m);
-    }
-    t.begin[e] = begin;
-    t.rows[e] = end - begin;
+    int begin, end;
+    expert_rows(p, e, begin, end);
+    t.first[e] = ((end - begin + tile_m - 1) / tile_m) * p.tiles_n;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
     int before = 0;
     for (int e0 = 0; e0 < p.experts; e0 += 32) {
       const int e = e0 + threadIdx.x;
-      const int own = e < p.experts ? ((t.rows[e] + tile_m - 1) / tile_m) * p.tiles_n : 0;
+      const int own = e < p.experts ? t.first[e] : 0;
       int sum = own;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -148,40 +154,68 @@ __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// One lane of a converged warp.  What this predicate guards the compiler knows to be one thread's, so that TMA and
+// tcgen05 operands go straight to uniform registers; behind `lane == 0` each such instruction becomes a loop
+// over the active lanes (about 90 cycles an MMA).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+// A bounded wait by a whole warp, with one answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const WaitCtx& wc) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, wc));
+}
+
 __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&w)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
 }
 
-// N features of one row, in order in acc (pairs), to dst; `valid` of them exist.
-template <typename Out, int N>
-__device__ __forceinline__ void store_features(Out* dst, const uint64_t* acc, int valid, bool wide) {
+// kN features of each of a warp's 32 rows (a lane each), in order in acc (pairs), to dst (the first row's, rows
+// `pitch` apart); `rows` and `valid` of them exist.  Rows that keep to 32 bytes are stored from the registers, whole
+// sectors at a time; others pass through shared memory, 16 columns at a time, and leave with the lanes along the row.
+template <typename Out, int kN>
+__device__ __forceinline__ void store_features(Out* dst, size_t pitch, const uint64_t* acc, int rows, int valid, bool wide,
+                                               float (*stage)[17], int lane) {
   constexpr int kPer = 32 / sizeof(Out);
+  if (wide) {
+    if (lane >= rows) return;
+    dst += lane * pitch;
 #pragma unroll
-  for (int g = 0; g < N / kPer; ++g) {
-    float f[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer / 2; ++i) {
-      const float2 v = unpack2(acc[g * (kPer / 2) + i]);
-      f[2 * i] = v.x;
-      f[2 * i + 1] = v.y;
-    }
-    if (wide && (g + 1) * kPer <= valid) {
+    for (int g = 0; g < kN / kPer; ++g) {
+      if ((g + 1) * kPer > valid) break;   // (rows are a multiple of 32 bytes, so is what is left)
       uint32_t w[8];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         float h[kPer / 2];
 #pragma unroll
-        for (int i = 0; i < kPer / 2; ++i) h[i] = f[q * (kPer / 2) + i];
+        for (int i = 0; i < kPer / 4; ++i) {
+          const float2 v = unpack2(acc[g * (kPer / 2) + q * (kPer / 4) + i]);
+          h[2 * i] = v.x;
+          h[2 * i + 1] = v.y;
+        }
         const uint4 u = pack16<Out>(h);
         w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
       }
       st_global_32(dst + g * kPer, w);
-    } else {
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (g * kPer + i < valid) dst[g * kPer + i] = from_float<Out>(f[i]);
+    for (int g = 0; g < kN / 16; ++g) {
+      if (g * 16 >= valid) break;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 v = unpack2(acc[g * 8 + i]);
+        stage[lane][2 * i] = v.x;
+        stage[lane][2 * i + 1] = v.y;
+      }
+      __syncwarp();
+      const int col = g * 16 + (lane & 15);
+      for (int r = lane >> 4; r < rows; r += 2)
+        if (col < valid) dst[r * pitch + col] = from_float<Out>(stage[r][lane & 15]);
+      __syncwarp();
     }
   }
 }
@@ -207,6 +241,7 @@ struct SharedTail {
   uint32_t abort_word;
   float scale[kScaleSlots][kScaleBlocks][2][128];   // [block of k][weight block][row]: a's scale times w's
   uint32_t amax[2][kColumnWarps][128];     // [tile parity]
+  float stage[kEpilogueWarps][32][17];     // output rows on their way, 16 columns at a time
   TileTable table;
 };
 
@@ -220,7 +255,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   extern __shared__ __align__(16) unsigned char s_raw[];
   unsigned char* ring = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);   // swizzle atoms are 1024 bytes
   SharedTail& sh = *reinterpret_cast<SharedTail*>(ring + kStages * kStageBytes);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // (uniform to the compiler)
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const WaitCtx wc{&sh.abort_word, p.spin_limit};
@@ -249,74 +284,62 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   if (warp < kEpilogueWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     if (warp == 0) {
-      if (lane == 0) {
-        // a plain MLP has no second weight tile: its follower loads the first one again, into columns nobody reads
-        const CUtensorMap* map_w = rank == 0 ? &map_w0 : &map_w1;
-        Ring at;
-        Tile t;
-        bool ok = true;
-        for (int i = pair; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += pairs) {
-          const int row = t.row0 + static_cast<int>(rank) * 128;
-          const int w_row = t.expert * p.n + t.n0 + (kGated ? 0 : static_cast<int>(rank) * 128);   // (fits: checked by the host)
-          for (int kb = 0; kb < p.kblocks; ++kb) {
-            if (!mbar_wait(&sh.done[at.stage], at.phase ^ 1, wc)) {
-              wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_EMPTY, i);
-              ok = false;
-              break;
-            }
+      // a plain MLP has no second weight tile: its follower loads the first one again, into columns nobody reads
+      const CUtensorMap* map_w = rank == 0 ? &map_w0 : &map_w1;
+      Ring at;
+      Tile t;
+      bool ok = true;
+      for (int i = pair; ok && find_tile(sh.table, p, i, kTileM, kTileN, t); i += pairs) {
+        const int row = t.row0 + static_cast<int>(rank) * 128;
+        const int w_row = t.expert * p.n + t.n0 + (kGated ? 0 : static_cast<int>(rank) * 128);   // (fits: checked by the host)
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          ok = warp_wait(&sh.done[at.stage], at.phase ^ 1, wc);
+          if (!ok) break;
+          if (elect_one()) {
             unsigned char* stage = ring + at.stage * kStageBytes;
             if (rank == 0) mbar_expect_tx(&sh.full[at.stage], 2 * kStageBytes);
             tma_load_2d_pair(stage, &map_a, &sh.full[at.stage], kb * kBlock, row);
             tma_load_2d_pair(stage + kBoxBytes, map_w, &sh.full[at.stage], kb * kBlock, w_row);
-            at.next();
           }
-        }
-        // no copy may be in flight when the CTA leaves: the MMAs that free a stage come after its copies
-        const WaitCtx last{nullptr, p.spin_limit};
-        for (int j = 0; j < kStages; ++j) {   // (a stage that was never filled passes at once)
-          mbar_wait(&sh.done[at.stage], at.phase ^ 1, last);
+          __syncwarp();
           at.next();
         }
+        if (!ok && lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_EMPTY, i);
+      }
+      // no copy may be in flight when the CTA leaves: the MMAs that free a stage come after its copies
+      const WaitCtx last{nullptr, p.spin_limit};
+      for (int j = 0; j < kStages; ++j) {   // (a stage that was never filled passes at once)
+        mbar_wait(&sh.done[at.stage], at.phase ^ 1, last);
+        at.next();
       }
     } else if (warp == 1) {
-      if (lane == 0 && rank == 0) {
+      if (rank == 0) {
         const uint32_t idesc = umma_idesc_e4m3(256, 256);
         const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
         Ring at;
-        int b = 0;
-        uint32_t b_phase = 1;
+        uint32_t b = 0, b_phase = 1, last_stage = 0, last_phase = 1;
         Tile t;
-        bool ok = true, ready = false;
-        uint32_t last_stage = 0, last_phase = 1;
-        for (int i = pair; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += pairs) {
+        bool ok = true;
+        for (int i = pair; ok && find_tile(sh.table, p, i, kTileM, kTileN, t); i += pairs) {
           for (int kb = 0; kb < p.kblocks; ++kb) {
-            if (!ready) {
-              if (!mbar_wait(&sh.acc_empty[b], b_phase, wc)) {
-                wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_EMPTY, i);
-                ok = false;
-                break;
-              }
-              if (!mbar_wait(&sh.full[at.stage], at.phase, wc)) {
-                wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_FULL, i);
-                ok = false;
-                break;
-              }
-            }
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.full[at.stage], at.phase, wc) && mbar_wait(&sh.acc_empty[b], b_phase, wc));
+            if (!ok) break;
             tc_fence_after_sync();
-            const uint64_t da = desc0 + at.stage * (kStageBytes >> 4), dw = da + (kBoxBytes >> 4);
-  #pragma unroll
-            for (int q = 0; q < 4; ++q)   // 32 bytes of k each
-              umma_f8_pair(tmem + b * 256, da + 2 * q, dw + 2 * q, idesc, q != 0);
-            umma_commit_pair(&sh.done[at.stage], 3);
+            if (elect_one()) {
+              const uint64_t da = desc0 + at.stage * (kStageBytes >> 4), dw = da + (kBoxBytes >> 4);
+#pragma unroll
+              for (int q = 0; q < 4; ++q)   // 32 bytes of k each
+                umma_f8_pair(tmem + b * 256, da + 2 * q, dw + 2 * q, idesc, q != 0);
+              umma_commit_pair(&sh.done[at.stage], 3);
+            }
+            __syncwarp();
             last_stage = at.stage;
             last_phase = at.phase;
             at.next();
             b ^= 1;
             b_phase ^= b == 0;
-            // look at the next block's barriers while the MMAs run
-            const bool f = mbar_try_wait(&sh.full[at.stage], at.phase), e = mbar_try_wait(&sh.acc_empty[b], b_phase);
-            ready = f && e;
           }
+          if (!ok && lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_FULL, i);
         }
         // no MMA may be running when TMEM is freed
         const WaitCtx last{nullptr, p.spin_limit};
@@ -329,7 +352,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       int done = 0;
       Tile t;
       bool ok = true;
-      for (int i = pair; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += pairs) {
+      for (int i = pair; ok && find_tile(sh.table, p, i, kTileM, kTileN, t); i += pairs) {
         const float* src[4] = {nullptr, nullptr, nullptr, nullptr};   // this lane's two rows, the two weight blocks
         for (int j = 0; j < 2; ++j) {
           const int row = t.row0 + static_cast<int>(rank) * 128 + r0 + 32 * j, nb = t.n0 / kBlock + (kGated ? 0 : j);
@@ -382,7 +405,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     int b = 0, groups = 0, parity = 0;
     Tile t;
     bool ok = true;
-    for (int i = pair; ok && find_tile(sh.table, p.experts, i, kTileM, kTileN, t); i += pairs, parity ^= 1) {
+    for (int i = pair; ok && find_tile(sh.table, p, i, kTileM, kTileN, t); i += pairs, parity ^= 1) {
       const int row = t.row0 + static_cast<int>(rank) * 128 + r;
       const bool live = row < t.row_end;
       uint64_t acc[kRun];   // pairs of columns: the first run's, then the second's
@@ -470,10 +493,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           }
           if (column_warp == 0) p.out_scale[static_cast<size_t>(row) * p.nblocks + t.n0 / kBlock] = block_scale(top);
         }
-      } else if (live) {
-        const int col = t.n0 + column0;
-        if (col < p.n)
-          store_features<Out, 2 * kRun>(static_cast<Out*>(p.out) + static_cast<size_t>(row) * p.n + col, acc, p.n - col, p.wide != 0);
+      } else {
+        const int col = t.n0 + column0, first_row = t.row0 + static_cast<int>(rank) * 128 + quarter * 32;
+        if (col < p.n && first_row < t.row_end)   // (the same for the whole warp)
+          store_features<Out, 2 * kRun>(static_cast<Out*>(p.out) + static_cast<size_t>(first_row) * p.n + col, p.n, acc,
+                                        min(32, t.row_end - first_row), p.n - col, p.wide != 0,
+                                        sh.stage[warp - kEpilogueWarp], lane);
       }
     }
   }
@@ -566,7 +591,7 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
   unsigned char* ring = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);
   float* sums = reinterpret_cast<float*>(ring + kStages * N::kStageBytes);   // [weight][row][feature], splits only
   auto& sh = *reinterpret_cast<typename N::Tail*>(ring + kStages * N::kStageBytes + N::kReduceBytes);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // (uniform to the compiler)
   const int splits = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_ctarank());
   const int first_tile = blockIdx.x / splits, tile_step = gridDim.x / splits;
   const int kb0 = p.kblocks * rank / splits, kb1 = p.kblocks * (rank + 1) / splits;   // this CTA's blocks of k
@@ -593,54 +618,45 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
   const bool second = kGated && p.has_v != 0;
 
   if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t bytes = N::kRowBytes + (second ? 2 : 1) * kBoxBytes;
-      uint32_t stage = 0, phase = 1;
-      Tile t;
-      bool ok = true;
-      for (int i = first_tile; ok && find_tile(sh.table, p.experts, i, kRows, kBlock, t); i += tile_step) {
-        const int w_row = t.expert * p.n + t.n0;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(&sh.done[stage], phase, wc)) {
-            wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_EMPTY, i);
-            ok = false;
-            break;
-          }
+    const uint32_t bytes = N::kRowBytes + (second ? 2 : 1) * kBoxBytes;
+    uint32_t stage = 0, phase = 1;
+    Tile t;
+    bool ok = true;
+    for (int i = first_tile; ok && find_tile(sh.table, p, i, kRows, kBlock, t); i += tile_step) {
+      const int w_row = t.expert * p.n + t.n0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = warp_wait(&sh.done[stage], phase, wc);
+        if (!ok) break;
+        if (elect_one()) {
           unsigned char* to = ring + stage * N::kStageBytes;
           mbar_expect_tx(&sh.full[stage], bytes);
           tma_load_2d(to, &map_w0, &sh.full[stage], kb * kBlock, w_row);
           if (second) tma_load_2d(to + kBoxBytes, &map_w1, &sh.full[stage], kb * kBlock, w_row);
           tma_load_2d(to + N::kWeights * kBoxBytes, &map_a, &sh.full[stage], kb * kBlock, t.row0);
-          if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
-      }
-      // no copy may be in flight when the CTA leaves: the MMAs that free a stage come after its copies
-      const WaitCtx last{nullptr, p.spin_limit};
-      for (int j = 0; j < kStages; ++j) {   // (a stage that was never filled passes at once)
-        mbar_wait(&sh.done[stage], phase, last);
+        __syncwarp();
         if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
+      if (!ok && lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_EMPTY, i);
+    }
+    // no copy may be in flight when the CTA leaves: the MMAs that free a stage come after its copies
+    const WaitCtx last{nullptr, p.spin_limit};
+    for (int j = 0; j < kStages; ++j) {   // (a stage that was never filled passes at once)
+      mbar_wait(&sh.done[stage], phase, last);
+      if (++stage == kStages) { stage = 0; phase ^= 1; }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = umma_idesc_e4m3(128, kRows);
-      const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
-      uint32_t stage = 0, phase = 0, b = 0, b_phase = 1, last_stage = 0, last_phase = 1;
-      Tile t;
-      bool ok = true;
-      for (int i = first_tile; ok && find_tile(sh.table, p.experts, i, kRows, kBlock, t); i += tile_step) {
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(&sh.acc_empty[b], b_phase, wc)) {
-            wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_EMPTY, i);
-            ok = false;
-            break;
-          }
-          if (!mbar_wait(&sh.full[stage], phase, wc)) {
-            wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_FULL, i);
-            ok = false;
-            break;
-          }
-          tc_fence_after_sync();
+    const uint32_t idesc = umma_idesc_e4m3(128, kRows);
+    const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
+    uint32_t stage = 0, phase = 0, b = 0, b_phase = 1, last_stage = 0, last_phase = 1;
+    Tile t;
+    bool ok = true;
+    for (int i = first_tile; ok && find_tile(sh.table, p, i, kRows, kBlock, t); i += tile_step) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.full[stage], phase, wc) && mbar_wait(&sh.acc_empty[b], b_phase, wc));
+        if (!ok) break;
+        tc_fence_after_sync();
+        if (elect_one()) {
           const uint64_t dw = desc0 + stage * (N::kStageBytes >> 4), da = dw + (N::kWeights * kBoxBytes >> 4);
           const uint32_t acc = tmem + b * N::kAccColumns;
 #pragma unroll
@@ -649,22 +665,24 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             if (second) umma_f8(acc + kRows, dw + (kBoxBytes >> 4) + 2 * q, da + 2 * q, idesc, q != 0);
           }
           umma_commit(&sh.done[stage]);
-          last_stage = stage;
-          last_phase = phase;
-          if (++stage == kStages) { stage = 0; phase ^= 1; }
-          if (++b == N::kAccs) { b = 0; b_phase ^= 1; }
         }
+        __syncwarp();
+        last_stage = stage;
+        last_phase = phase;
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
+        if (++b == N::kAccs) { b = 0; b_phase ^= 1; }
       }
-      const WaitCtx last{nullptr, p.spin_limit};
-      mbar_wait(&sh.done[last_stage], last_phase, last);   // no MMA may be running when TMEM is freed
+      if (!ok && lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_FULL, i);
     }
+    const WaitCtx last{nullptr, p.spin_limit};
+    mbar_wait(&sh.done[last_stage], last_phase, last);   // no MMA may be running when TMEM is freed
   } else if (warp == kScaleWarp) {
     // each lane up to four rows, four blocks of k at a time, four to eight blocks ahead
     constexpr int kLaneRows = kRows < 32 ? 1 : kRows / 32;
     int groups = 0;
     Tile t;
     bool ok = true;
-    for (int i = first_tile; ok && find_tile(sh.table, p.experts, i, kRows, kBlock, t); i += tile_step) {
+    for (int i = first_tile; ok && find_tile(sh.table, p, i, kRows, kBlock, t); i += tile_step) {
       const size_t w_at = (static_cast<size_t>(t.expert) * p.nblocks + t.n0 / kBlock) * p.kblocks;
       const float* w[2] = {p.w_scale[0] + w_at, second ? p.w_scale[1] + w_at : p.w_scale[0] + w_at};
       float a_next[kLaneRows][4], w_next[2][4];
@@ -716,7 +734,7 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     int groups = 0, parity = 0;
     Tile t;
     bool ok = true;
-    for (int i = first_tile; ok && find_tile(sh.table, p.experts, i, kRows, kBlock, t); i += tile_step, parity ^= 1) {
+    for (int i = first_tile; ok && find_tile(sh.table, p, i, kRows, kBlock, t); i += tile_step, parity ^= 1) {
       const int feature = t.n0 + quarter * 32 + lane;
       uint64_t acc[N::kWeights][kPart / 2];   // pairs of rows
 #pragma unroll
@@ -805,20 +823,19 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         if (lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TMEM_FULL, i);
         break;
       }
-      const int row0 = t.row0 + half * kPart + from;
+      const int row0 = t.row0 + half * kPart + from, live = min(count, t.row_end - row0);   // (may be none)
       if constexpr (kGated) {
         uint32_t* amax = sh.amax[parity][half * 4 + quarter];
 #pragma unroll
-        for (int j = 0; j < kPart / 2; ++j) {
-          const float2 g = unpack2(acc[0][j]), u = unpack2(acc[1][j]);
-          float h0 = activate(g.x, p.act), h1 = activate(g.y, p.act);
-          if (second) { h0 *= u.x; h1 *= u.y; }
-          if (feature >= p.n) h0 = h1 = 0.0f;
-          acc[0][j] = pack2(h0, h1);
-          const uint32_t m0 = __reduce_max_sync(0xffffffffu, abs_bits(h0)), m1 = __reduce_max_sync(0xffffffffu, abs_bits(h1));
-          if (lane == 0) {
-            amax[2 * j] = m0;
-            amax[2 * j + 1] = m1;
+        for (int j = 0; j < kPart; ++j) {
+          if (j < live) {   // (the same for the whole warp)
+            const float2 g = unpack2(acc[0][j / 2]), u = unpack2(acc[1][j / 2]);
+            float h = activate(j & 1 ? g.y : g.x, p.act);
+            if (second) h *= j & 1 ? u.y : u.x;
+            if (feature >= p.n) h = 0.0f;
+            acc[0][j / 2] = j & 1 ? pack2(g.x, h) : pack2(h, g.y);
+            const uint32_t m = __reduce_max_sync(0xffffffffu, abs_bits(h));
+            if (lane == 0) amax[j] = m;
           }
         }
         __syncwarp();
@@ -828,27 +845,41 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
           if (lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_TASK, i);
           break;
         }
+        // each lane works out the scales of every 32nd row and hands them round
+        float inv[(kPart + 31) / 32], pre[(kPart + 31) / 32];
 #pragma unroll
-        for (int j = 0; j < kPart; ++j) {
-          const int row = row0 + j;
-          if (j < count && row < t.row_end) {
-            uint32_t m = 0;
+        for (int c = 0; c < (kPart + 31) / 32; ++c) {
+          const int j = c * 32 + lane;
+          uint32_t m = 0;
+          if (j < live) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) m = max(m, sh.amax[parity][half * 4 + q][j]);
-            const float top = __uint_as_float(m);
+            if (quarter == 0) p.out_scale[static_cast<size_t>(row0 + j) * p.nblocks + t.n0 / kBlock] = block_scale(__uint_as_float(m));
+          }
+          const FastQuantizer z(__uint_as_float(m));
+          inv[c] = z.inv;
+          pre[c] = z.pre;
+        }
+        unsigned char* to = static_cast<unsigned char*>(p.out) + static_cast<size_t>(row0) * p.n + feature;
+#pragma unroll
+        for (int j = 0; j < kPart; ++j) {
+          if (j < live) {
             const float2 v = unpack2(acc[0][j / 2]);
-            const float h = FastQuantizer(top).scaled(j & 1 ? v.y : v.x);
-            if (feature < p.n)
-              static_cast<unsigned char*>(p.out)[static_cast<size_t>(row) * p.n + feature] = static_cast<unsigned char>(to_e4m3x2(h, 0.0f));
-            if (quarter == 0 && lane == 0) p.out_scale[static_cast<size_t>(row) * p.nblocks + t.n0 / kBlock] = block_scale(top);
+            const float a = __shfl_sync(0xffffffffu, pre[j / 32], j & 31), f = __shfl_sync(0xffffffffu, inv[j / 32], j & 31);
+            const uint32_t code = to_e4m3x2(((j & 1) ? v.y : v.x) * a * f, 0.0f);
+            if (feature < p.n) *to = static_cast<unsigned char>(code);
+            to += p.n;
           }
         }
       } else if (feature < p.n) {
         Out* to = static_cast<Out*>(p.out) + static_cast<size_t>(row0) * p.n + feature;
 #pragma unroll
         for (int j = 0; j < kPart; ++j) {
-          const float2 v = unpack2(acc[0][j / 2]);
-          if (j < count && row0 + j < t.row_end) to[static_cast<size_t>(j) * p.n] = from_float<Out>(j & 1 ? v.y : v.x);
+          if (j < live) {
+            const float2 v = unpack2(acc[0][j / 2]);
+            *to = from_float<Out>(j & 1 ? v.y : v.x);
+            to += p.n;
+          }
         }
       }
     }
