@@ -35,8 +35,6 @@ constexpr int kRun = 128 / kColumnWarps;   // columns of one weight block that a
 constexpr int kLoadRegs = 88, kEpilogueRegs = 208;
 constexpr int kMaxExperts = 1024;
 constexpr uint32_t kBoxBytes = 128 * kBlock;   // 128 rows of one k block: 16 KB
-constexpr int kStages = 6;
-constexpr uint32_t kStageBytes = 2 * kBoxBytes;   // 128 rows of each operand
 
 struct Codes {};   // "output type" of the gated form
 
@@ -221,6 +219,7 @@ __device__ __forceinline__ void store_features(Out* dst, size_t pitch, const uin
 }
 
 // A place in the ring of stages, and the parity of the round it is in.
+template <int kStages>
 struct Ring {
   uint32_t stage = 0, phase = 0;
   __device__ __forceinline__ void next() {
@@ -231,7 +230,16 @@ struct Ring {
   }
 };
 
-struct SharedTail {
+// A pair's CTA holds 128 rows of each operand, a CTA alone 128 rows and 256 features.
+template <bool kPair>
+struct Wide {
+  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr uint32_t kStageBytes = (kPair ? 2 : 3) * kBoxBytes;
+  struct Tail;
+  static constexpr size_t smem_bytes();
+};
+template <bool kPair>
+struct Wide<kPair>::Tail {
   uint64_t full[kStages];         // the leader's: both CTAs' copies of the stage have landed
   uint64_t done[kStages];         // each CTA's: the MMAs of the stage are done: it is free, its sums are in TMEM
   uint64_t acc_empty[2];          // the leader's: both CTAs have read it
@@ -244,25 +252,31 @@ struct SharedTail {
   float stage[kEpilogueWarps][32][17];     // output rows on their way, 16 columns at a time
   TileTable table;
 };
+template <bool kPair>
+constexpr size_t Wide<kPair>::smem_bytes() { return 1024 + kStages * kStageBytes + sizeof(Tail); }
+static_assert(Wide<true>::smem_bytes() <= 227 * 1024 && Wide<false>::smem_bytes() <= 227 * 1024, "shared memory of one CTA");
 
 // Rows on the TMEM lanes, features on its columns.
-template <typename Out>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+template <typename Out, bool kPair>
+__global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w0,
                const __grid_constant__ CUtensorMap map_w1, const ProductParams p) {
   constexpr bool kGated = std::is_same_v<Out, Codes>;
-  constexpr int kTileM = 256, kTileN = kGated ? 128 : 256;
+  constexpr int kCtas = kPair ? 2 : 1, kTileM = 128 * kCtas, kTileN = kGated ? 128 : 256;
+  using W = Wide<kPair>;
+  constexpr int kStages = W::kStages;
+  constexpr uint32_t kStageBytes = W::kStageBytes;
   extern __shared__ __align__(16) unsigned char s_raw[];
   unsigned char* ring = s_raw + ((1024 - (smem_u32(s_raw) & 1023)) & 1023);   // swizzle atoms are 1024 bytes
-  SharedTail& sh = *reinterpret_cast<SharedTail*>(ring + kStages * kStageBytes);
+  auto& sh = *reinterpret_cast<typename W::Tail*>(ring + kStages * kStageBytes);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // (uniform to the compiler)
-  const uint32_t rank = cluster_ctarank();
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t rank = kPair ? cluster_ctarank() : 0;
+  const int pair = blockIdx.x / kCtas, pairs = gridDim.x / kCtas;
   const WaitCtx wc{&sh.abort_word, p.spin_limit};
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.done[i], 1); }
-    for (int i = 0; i < 2; ++i) mbar_init(&sh.acc_empty[i], 2 * kEpilogueWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.acc_empty[i], kCtas * kEpilogueWarps);
     for (int i = 0; i < 4; ++i) mbar_init(&sh.amax_full[i], kColumnWarps);
     for (int i = 0; i < kScaleSlots; ++i) {
       mbar_init(&sh.scale_full[i], kScaleWarps);
@@ -272,11 +286,16 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     mbar_fence_init();
   }
   if (warp == 1) {
-    tmem_alloc_pair(&sh.tmem_base, 512);
-    tmem_relinquish_pair();
+    if constexpr (kPair) {
+      tmem_alloc_pair(&sh.tmem_base, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&sh.tmem_base, 512);
+      tmem_relinquish();
+    }
   }
   fill_table(sh.table, p, kTileM);
-  cluster_sync_all();   // both CTAs' barriers exist before either is signalled from the other
+  if constexpr (kPair) cluster_sync_all();   // both CTAs' barriers exist before either is signalled from the other
   tc_fence_after_sync();
   const uint32_t tmem = sh.tmem_base;
   const bool second = !kGated || p.has_v != 0;   // whether the second 128 weight rows exist
@@ -286,7 +305,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (warp == 0) {
       // a plain MLP has no second weight tile: its follower loads the first one again, into columns nobody reads
       const CUtensorMap* map_w = rank == 0 ? &map_w0 : &map_w1;
-      Ring at;
+      Ring<kStages> at;
       Tile t;
       bool ok = true;
       for (int i = pair; ok && find_tile(sh.table, p, i, kTileM, kTileN, t); i += pairs) {
@@ -297,9 +316,17 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           if (!ok) break;
           if (elect_one()) {
             unsigned char* stage = ring + at.stage * kStageBytes;
-            if (rank == 0) mbar_expect_tx(&sh.full[at.stage], 2 * kStageBytes);
-            tma_load_2d_pair(stage, &map_a, &sh.full[at.stage], kb * kBlock, row);
-            tma_load_2d_pair(stage + kBoxBytes, map_w, &sh.full[at.stage], kb * kBlock, w_row);
+            if constexpr (kPair) {
+              if (rank == 0) mbar_expect_tx(&sh.full[at.stage], 2 * kStageBytes);
+              tma_load_2d_pair(stage, &map_a, &sh.full[at.stage], kb * kBlock, row);
+              tma_load_2d_pair(stage + kBoxBytes, map_w, &sh.full[at.stage], kb * kBlock, w_row);
+            } else {
+              mbar_expect_tx(&sh.full[at.stage], (second ? 3 : 2) * kBoxBytes);
+              tma_load_2d(stage, &map_a, &sh.full[at.stage], kb * kBlock, row);
+              tma_load_2d(stage + kBoxBytes, &map_w0, &sh.full[at.stage], kb * kBlock, w_row);
+              if (second)
+                tma_load_2d(stage + 2 * kBoxBytes, &map_w1, &sh.full[at.stage], kb * kBlock, kGated ? w_row : w_row + 128);
+            }
           }
           __syncwarp();
           at.next();
@@ -314,9 +341,9 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       }
     } else if (warp == 1) {
       if (rank == 0) {
-        const uint32_t idesc = umma_idesc_e4m3(256, 256);
+        const uint32_t idesc = kPair ? umma_idesc_e4m3(256, 256) : umma_idesc_e4m3(128, second ? 256 : 128);
         const uint64_t desc0 = umma_desc_sw128(smem_u32(ring));
-        Ring at;
+        Ring<kStages> at;
         uint32_t b = 0, b_phase = 1, last_stage = 0, last_phase = 1;
         Tile t;
         bool ok = true;
@@ -328,9 +355,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             if (elect_one()) {
               const uint64_t da = desc0 + at.stage * (kStageBytes >> 4), dw = da + (kBoxBytes >> 4);
 #pragma unroll
-              for (int q = 0; q < 4; ++q)   // 32 bytes of k each
-                umma_f8_pair(tmem + b * 256, da + 2 * q, dw + 2 * q, idesc, q != 0);
-              umma_commit_pair(&sh.done[at.stage], 3);
+              for (int q = 0; q < 4; ++q) {   // 32 bytes of k each
+                if constexpr (kPair) umma_f8_pair(tmem + b * 256, da + 2 * q, dw + 2 * q, idesc, q != 0);
+                else umma_f8(tmem + b * 256, da + 2 * q, dw + 2 * q, idesc, q != 0);
+              }
+              if constexpr (kPair) umma_commit_pair(&sh.done[at.stage], 3);
+              else umma_commit(&sh.done[at.stage]);
             }
             __syncwarp();
             last_stage = at.stage;
@@ -400,14 +430,18 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const int block0 = kGated ? 0 : column_warp * 2 / kColumnWarps, block1 = kGated ? 1 : block0;
     const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + column0;
     const int r = quarter * 32 + lane;
-    const uint32_t acc_empty[2] = {map_to_cta(&sh.acc_empty[0], 0), map_to_cta(&sh.acc_empty[1], 0)};
-    Ring at;
+    uint32_t acc_empty[2] = {0, 0};
+    if constexpr (kPair) {
+      acc_empty[0] = map_to_cta(&sh.acc_empty[0], 0);
+      acc_empty[1] = map_to_cta(&sh.acc_empty[1], 0);
+    }
+    Ring<kStages> at;
     int b = 0, groups = 0, parity = 0;
     Tile t;
     bool ok = true;
     for (int i = pair; ok && find_tile(sh.table, p, i, kTileM, kTileN, t); i += pairs, parity ^= 1) {
       const int row = t.row0 + static_cast<int>(rank) * 128 + r;
-      const bool live = row < t.row_end;
+      const bool live = row < t.row_end, any_live = row - lane < t.row_end;   // (any: the same for the whole warp)
       uint64_t acc[kRun];   // pairs of columns: the first run's, then the second's
 #pragma unroll
       for (int j = 0; j < kRun; ++j) acc[j] = 0;
@@ -422,28 +456,33 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         __syncwarp();
         tc_fence_after_sync();
         const uint64_t s0 = pack2(f0, f0), s1 = kGated ? pack2(f1, f1) : s0;
+        // chunk by chunk; the accumulator goes back as soon as the last one has been read (the branch over rows that do
+        // not exist pays where tiles are half empty; in the pair kernel it costs 6 % of 8192^3)
         uint32_t d[16];
+        auto add = [&](int c) {
 #pragma unroll
-        for (int c = 0; c < kChunks - 1; ++c) {
-          tmem_ld_16(taddr + b * 256 + column(c), d);
-          tmem_wait_16(d);
+          for (int j = 0; j < 8; ++j)
+            acc[c * 8 + j] = fma2(pack2(d[2 * j], d[2 * j + 1]), c < kChunks / 2 ? s0 : s1, acc[c * 8 + j]);
+        };
+        if (kPair || any_live) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) acc[c * 8 + j] = fma2(pack2(d[2 * j], d[2 * j + 1]), c < kChunks / 2 ? s0 : s1, acc[c * 8 + j]);
+          for (int c = 0; c < kChunks; ++c) {
+            tmem_ld_16(taddr + b * 256 + column(c), d);
+            tmem_wait_16(d);
+            if (c + 1 < kChunks) add(c);
+          }
         }
-        tmem_ld_16(taddr + b * 256 + column(kChunks - 1), d);
-        tmem_wait_16(d);
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) arrive_at(acc_empty[b]);
+        if (lane == 0) {
+          if constexpr (kPair) arrive_at(acc_empty[b]);
+          else mbar_arrive(&sh.acc_empty[b]);
+        }
         if (x == kScaleBlocks - 1 || kb + 1 == p.kblocks) {
           if (lane == 0) mbar_arrive(&sh.scale_empty[slot]);
           ++groups;
         }
-        {
-          constexpr int c = kChunks - 1;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) acc[c * 8 + j] = fma2(pack2(d[2 * j], d[2 * j + 1]), c < kChunks / 2 ? s0 : s1, acc[c * 8 + j]);
-        }
+        if (kPair || any_live) add(kChunks - 1);
         at.next();
         b ^= 1;
       }
@@ -503,8 +542,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
   }
   __syncthreads();
-  cluster_sync_all();   // nothing of this CTA's is signalled from the other any more
-  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+  if constexpr (kPair) {
+    cluster_sync_all();   // nothing of this CTA's is signalled from the other any more
+    if (warp == 1) tmem_dealloc_pair(tmem, 512);
+  } else if (warp == 1) {
+    tmem_dealloc(tmem, 512);
+  }
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------
@@ -889,9 +932,6 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
   if (warp == 1) tmem_dealloc(tmem, N::kTmemColumns);
 }
 
-constexpr size_t kProductSmem = 1024 + kStages * kStageBytes + sizeof(SharedTail);
-static_assert(kProductSmem <= 227 * 1024, "shared memory of one CTA");
-
 // What a launch needs to know about a device, looked up once.
 struct DeviceFacts {
   int sms = 0;
@@ -909,7 +949,7 @@ const DeviceFacts& facts(int device) {
   return all[device];
 }
 
-// Launches a kernel in clusters of `cluster` CTAs (0: its own compile-time shape).
+// Launches a kernel in clusters of `cluster` CTAs.
 template <typename Kernel>
 int launch_kernel(Kernel kernel, std::atomic<unsigned long long>& prepared, size_t smem, int threads, int grid, int cluster,
                   const CUtensorMap (&maps)[3], const ProductParams& p, int device, cudaStream_t stream) {
@@ -936,10 +976,11 @@ int launch_kernel(Kernel kernel, std::atomic<unsigned long long>& prepared, size
   return FMOE_OK;
 }
 
-template <typename Out>
+template <typename Out, bool kPair>
 int launch_wide(const ProductParams& p, const CUtensorMap (&maps)[3], int grid, int device, cudaStream_t stream) {
   static std::atomic<unsigned long long> prepared{0};
-  return launch_kernel(product_kernel<Out>, prepared, kProductSmem, kThreads, grid, 0, maps, p, device, stream);
+  return launch_kernel(product_kernel<Out, kPair>, prepared, Wide<kPair>::smem_bytes(), kThreads, grid, kPair ? 2 : 1, maps, p,
+                       device, stream);
 }
 template <typename Out, int kRows>
 int launch_narrow(const ProductParams& p, const CUtensorMap (&maps)[3], int grid, int splits, int device, cudaStream_t stream) {
@@ -951,45 +992,65 @@ int launch_narrow(const ProductParams& p, const CUtensorMap (&maps)[3], int grid
 
 // Which kernel a product takes, and its launch shape.
 struct Shape {
-  int rows;     // rows a tile has: 256 (pairs), or 16, 32, 64, 128 (few rows)
+  int rows;     // rows a tile has: 256 (pairs), 128 (a CTA alone), or 16, 32, 64 (few rows)
   int splits;   // CTAs that share a tile (few rows only)
   int grid;
 };
 
-Shape shape_for(int m, int features, int kblocks, int experts, int features_wide, int sms) {
-  Shape s{256, 1, 0};
-  const int hit = experts > 1 ? (m < experts ? m : experts) : 1;
-  const double mean = static_cast<double>(m) / hit;
-  if (mean <= 12 || (experts == 1 && m <= 16)) s.rows = 16;
-  else if (mean <= 24 || (experts == 1 && m <= 32)) s.rows = 32;
-  else if (mean <= 48 || (experts == 1 && m <= 64)) s.rows = 64;
-  else if (mean <= 128) s.rows = 128;
-  const int tile_n = s.rows == 256 ? features_wide : kBlock;
-  const long long tiles_n = (features + tile_n - 1) / tile_n;
-  // at most this many tiles (how the rows spread over the experts is known on the device only)
-  const long long tiles = (m / s.rows + hit) * tiles_n;
-  if (s.rows == 256) {
-    const long long pairs = sms / 2;
-    s.grid = 2 * static_cast<int>(tiles < pairs ? tiles : pairs);
-    return s;
+// The kernels differ in how much of a tile they can keep busy, so the choice goes by waves of tiles times what a block
+// of k of one tile takes, measured (k = 4096, 8192 features, 24 to 2560 rows; and 8 and 128 experts of 12 to 1024
+// rows): about 0.24 us for 16 and 32 rows x 128 features, 0.32 for 64 x 128, 0.62 for 128 x 256, 0.58 for the
+// pair's 256 x 256, whose launch takes some 3 us more; outputs whose rows are no multiple of 32 bytes cost the last
+// two another 5 us.  (640 rows: 51, 36.9 and 39.4 us by 64, 128 and 256 rows; 8 experts of 1024: 952, 645, 607 us.)
+Shape shape_for(int m, int features, int kblocks, int experts, bool gated, bool wide_rows, int sms) {
+  struct Kind { int rows; double block, fixed; };
+  const int features_wide = gated ? 128 : 256;
+  const double odd = wide_rows ? 0.0 : 5.0, twice = gated ? 2.0 : 1.0;   // (128 features of two weights)
+  const Kind kinds[] = {{16, 0.24 * twice, 0.0}, {32, 0.24 * twice, 0.0}, {64, 0.32 * twice, 0.0}, {128, 0.62, odd},
+                        {256, 0.58, odd + 3.0}};
+  const int hit = experts > 1 ? (m < experts ? m : experts) : 1;   // experts that can have rows
+  Shape best{0, 1, 0};
+  double least = 0.0;
+  for (const Kind& kind : kinds) {
+    const int tile_n = kind.rows >= 128 ? features_wide : kBlock;
+    const int slots = kind.rows == 256 ? sms / 2 : sms;            // tiles at work at a time
+    const long long tiles_n = (features + tile_n - 1) / tile_n;
+    // How the rows spread over the experts is known on the device only: at most `most` tiles, and with rows spread
+    // at random around the mean half a tile more than the mean fills.
+    const long long most = (experts > 1 ? m / kind.rows + hit : (m + kind.rows - 1) / kind.rows) * tiles_n;
+    double tiles = static_cast<double>(most);
+    if (experts > 1) {
+      const double each = static_cast<double>(m) / hit / kind.rows + 0.5;
+      tiles = (each < 1.0 ? 1.0 : each) * hit * tiles_n;
+    }
+    Shape s{kind.rows, 1, 0};
+    while (s.rows <= 32 && s.splits < kMaxSplits && 2 * s.splits <= s.rows / 2 && 2 * s.splits * most <= sms &&
+           kblocks >= 8 * s.splits)
+      s.splits *= 2;
+    double waves = tiles * s.splits / slots;
+    if (experts == 1) waves = static_cast<double>((most * s.splits + slots - 1) / slots);
+    if (waves < 1.0) waves = 1.0;
+    const double cost = waves * kblocks / s.splits * kind.block + kind.fixed;
+    const long long ctas = kind.rows == 256 ? 2 * (most < slots ? most : slots)
+                                            : s.splits * (most < slots / s.splits ? most : slots / s.splits);
+    s.grid = static_cast<int>(ctas);
+    if (best.rows == 0 || cost < least) {
+      best = s;
+      least = cost;
+    }
   }
-  while (s.rows <= 32 && s.splits < kMaxSplits && 2 * s.splits <= s.rows / 2 && tiles * s.splits * 2 <= sms &&
-         kblocks >= 8 * s.splits)
-    s.splits *= 2;
-  const long long most = sms / s.splits;
-  s.grid = s.splits * static_cast<int>(tiles < most ? tiles : most);
-  return s;
+  return best;
 }
 
 template <typename Out>
 int launch_product(ProductParams p, const void* a, const void* w0, const void* w1, int device, cudaStream_t stream) {
   constexpr int kWideN = std::is_same_v<Out, Codes> ? 128 : 256;
-  const Shape s = shape_for(p.m, p.n, p.kblocks, p.experts, kWideN, facts(device).sms);
-  const int tile_n = s.rows == 256 ? kWideN : kBlock;
+  const Shape s = shape_for(p.m, p.n, p.kblocks, p.experts, std::is_same_v<Out, Codes>, std::is_same_v<Out, Codes> || p.wide != 0, facts(device).sms);
+  const int tile_n = s.rows >= 128 ? kWideN : kBlock;
   p.tiles_n = (p.n + tile_n - 1) / tile_n;
   CUtensorMap maps[3];
   const uint64_t w_rows = static_cast<uint64_t>(p.experts) * p.n;
-  int rc = make_byte_map(&maps[0], a, p.m, p.k, s.rows == 256 ? 128 : s.rows);
+  int rc = make_byte_map(&maps[0], a, p.m, p.k, s.rows >= 128 ? 128 : s.rows);
   if (rc == FMOE_OK) rc = make_byte_map(&maps[1], w0, w_rows, p.k, 128);
   if (rc == FMOE_OK && w1 != w0) rc = make_byte_map(&maps[2], w1, w_rows, p.k, 128);
   if (rc != FMOE_OK) return rc;
@@ -998,8 +1059,8 @@ int launch_product(ProductParams p, const void* a, const void* w0, const void* w
     case 16: return launch_narrow<Out, 16>(p, maps, s.grid, s.splits, device, stream);
     case 32: return launch_narrow<Out, 32>(p, maps, s.grid, s.splits, device, stream);
     case 64: return launch_narrow<Out, 64>(p, maps, s.grid, s.splits, device, stream);
-    case 128: return launch_narrow<Out, 128>(p, maps, s.grid, s.splits, device, stream);
-    default: return launch_wide<Out>(p, maps, s.grid, device, stream);
+    case 128: return launch_wide<Out, false>(p, maps, s.grid, device, stream);
+    default: return launch_wide<Out, true>(p, maps, s.grid, device, stream);
   }
 }
 
