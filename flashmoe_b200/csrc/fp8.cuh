@@ -19,21 +19,60 @@ constexpr float kE4m3Max = 448.0f;   // largest finite e4m3 value
 
 __host__ __device__ constexpr int blocks_of(int n) { return (n + kBlock - 1) / kBlock; }
 
+// ---- pairs of fp32 ---------------------------------------------------------------------------
+// Two independent operations an instruction, each rounded as a scalar one.
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+
 // ---- quantisation arithmetic ----------------------------------------------------------------
 // scale = amax / 448, code = e4m3(448 x / amax), all in IEEE fp32.  For 16-bit x the product 448 x
 // is exact and the quotient correctly rounded, so the code is the one infinite precision would give:
 // a quotient of two such numbers that is not a midpoint of two codes is at least 2^-11 of itself away
 // from one, far more than half an fp32 step.
-// Very large blocks are scaled down by a power of two first (448 x must stay finite); values that
-// underflow by it are below 2^-200 of amax and have the code 0 either way.
+// The quotient is taken with the reciprocal and one correction, y = n r, y + r (n - y d): with r = 1 / d correctly
+// rounded the result is the correctly rounded n / d (P. Markstein, Computation of elementary functions on the IBM
+// RISC System/6000 processor, 1990), at four operations a value, two values to an instruction; a division
+// instruction per value made the kernel wait for arithmetic at half the memory's rate.
+// Very large and very small blocks are scaled by a power of two first, so that 448 x stays finite and 1 / d
+// exists; values that underflow by it are below 2^-200 of amax and have the code 0 either way.
 struct Quantizer {
-  float num, den;   // code = e4m3((num x) / den)
+  uint64_t num, neg_den, rcp;   // pairs
   __device__ __forceinline__ explicit Quantizer(float amax) {
-    const float pre = amax > 0x1p+100f ? 0x1p-20f : 1.0f;
-    num = kE4m3Max * pre;
-    den = amax > 0.0f ? amax * pre : (amax == 0.0f ? 1.0f : amax);   // an empty block: codes 0; NaN stays
+    const float pre = amax > 0x1p+100f ? 0x1p-20f : (amax < 0x1p-100f ? 0x1p+100f : 1.0f);
+    const float den = amax > 0.0f ? amax * pre : (amax == 0.0f ? 1.0f : amax);   // an empty block: codes 0; NaN stays
+    const float n = kE4m3Max * pre, r = __frcp_rn(den);
+    num = pack2(n, n);
+    neg_den = pack2(-den, -den);
+    rcp = pack2(r, r);
   }
-  __device__ __forceinline__ float scaled(float x) const { return __fdiv_rn(__fmul_rn(x, num), den); }
+  // 448 x / amax of two values
+  __device__ __forceinline__ float2 scaled(float a, float b) const {
+    const uint64_t n = mul2(pack2(a, b), num), y = mul2(n, rcp);
+    return unpack2(fma2(fma2(y, neg_den, n), rcp, y));
+  }
 };
 // The same for values that carry rounding errors of their own (a product's results): one division per
 // block, then a product per value, at most 2^-23 from the quotient.
@@ -154,28 +193,6 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64
       ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Two independent fp32 multiply-adds.
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-
 // ---- host side -----------------------------------------------------------------------------------
 // Makes `device` current for the scope and puts the caller's device back.
 struct OnDevice {

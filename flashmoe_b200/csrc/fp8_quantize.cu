@@ -32,7 +32,28 @@ struct Raw16 {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) u[i] = make_uint4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ void values(float (&f)[16]) const {
+  // The largest |x|, as bits that order like the value (16-bit types: their own bits, two at a time).
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) m = max(m, w[j] & 0x7fffffffu);
+        else m = __vmaxu2(m, w[j] & 0x7fff7fffu);
+      }
+    }
+    if constexpr (sizeof(T) == 2) m = max(m & 0xffffu, m >> 16);
+    return m;
+  }
+  __device__ __forceinline__ static float amax_value(uint32_t bits) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(bits);
+    else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(bits << 16);
+    else return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+  }
+  __device__ __forceinline__ uint4 codes(const Quantizer& z) const {
+    float f[16];
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       float part[kPer];
@@ -40,22 +61,12 @@ struct Raw16 {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) f[i * kPer + j] = part[j];
     }
-  }
-  __device__ __forceinline__ uint32_t amax() const {
-    float f[16];
-    values(f);
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m = max(m, abs_bits(f[i]));
-    return m;
-  }
-  __device__ __forceinline__ uint4 codes(const Quantizer& z) const {
-    float f[16];
-    values(f);
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = to_e4m3x4(z.scaled(f[4 * i]), z.scaled(f[4 * i + 1]), z.scaled(f[4 * i + 2]), z.scaled(f[4 * i + 3]));
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = z.scaled(f[4 * i], f[4 * i + 1]), b = z.scaled(f[4 * i + 2], f[4 * i + 3]);
+      w[i] = to_e4m3x4(a.x, a.y, b.x, b.y);
+    }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
@@ -63,18 +74,19 @@ struct Raw16 {
 // Eight threads a block of 128, sixteen values each.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams p) {
-  const long long block = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 3;
+  const uint32_t block = blockIdx.x * (256 / 8) + (threadIdx.x >> 3);   // (the host sees to it that it fits)
   const int sub = threadIdx.x & 7;
-  const long long row = block / p.col_blocks;
-  const int cb = static_cast<int>(block - row * p.col_blocks), col = cb * kBlock + sub * 16;
+  const uint32_t row32 = block / static_cast<uint32_t>(p.col_blocks);
+  const long long row = row32;
+  const int cb = static_cast<int>(block - row32 * p.col_blocks), col = cb * kBlock + sub * 16;
   const bool in = row < p.rows && col < p.cols;   // (cols is a multiple of 16)
   Raw16<T> raw;
   raw.zero();
   if (in) raw.load(static_cast<const T*>(p.x) + row * p.cols + col);
-  uint32_t m = raw.amax();
+  uint32_t m = raw.amax_bits();
 #pragma unroll
   for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-  const float amax = __uint_as_float(m);
+  const float amax = Raw16<T>::amax_value(m);
   const uint4 codes = raw.codes(Quantizer(amax));
   if (row >= p.rows) return;
   for (int j = 0; j < p.copies; ++j) {
@@ -105,13 +117,13 @@ __global__ void __launch_bounds__(256) quantize_weights_kernel(const QuantizePar
       raw[i].load(static_cast<const T*>(p.x) + base + static_cast<size_t>(row0 + 32 * i) * p.cols);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m = max(m, raw[i].amax());
+  for (int i = 0; i < 4; ++i) m = max(m, raw[i].amax_bits());
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, s_max[i]);
-  const float amax = __uint_as_float(m);
+  const float amax = Raw16<T>::amax_value(m);
   const Quantizer z(amax);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -170,7 +182,7 @@ extern "C" int fmoe_fp8_quantize(const fmoe_fp8_quantize_args* a, void* stream) 
     p.rows *= matrices;
     p.row_blocks = p.rows;
     matrices = 1;
-    if (static_cast<long long>(p.rows) * p.col_blocks * 8 / 256 >= 0x7fffffffll)
+    if (static_cast<long long>(p.rows) * p.col_blocks > 0xffffff00ll)
       return set_error(FMOE_ERR_UNSUPPORTED, "more blocks than a grid holds");
   } else if (matrices > 65535 || static_cast<long long>(p.row_blocks) * p.col_blocks > 0x7fffffffll) {
     return set_error(FMOE_ERR_UNSUPPORTED, "at most 65535 matrices, and blocks of one must fit 32 bits");

@@ -37,6 +37,11 @@ struct SelectParams {
   float scale;
 };
 
+// Programmatic launches: the next grid may start when every CTA of this one has said so, and waits for this one's
+// results where it needs them.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- choosing ---------------------------------------------------------------------------------------
 
 // A masked expert (-infinity or NaN) orders below every other; +infinity is the largest finite number.
@@ -260,38 +265,81 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
 #pragma unroll
     for (int i = 0; i < V; ++i) c[i] = v[i];
   }
-  uint32_t alive = alive_bits<V>(p.E, p.groups, kept, lane);
+  const uint32_t alive = alive_bits<V>(p.E, p.groups, kept, lane);
+  uint32_t keys[V];   // 0: not there, or taken
+#pragma unroll
+  for (int i = 0; i < V; ++i) keys[i] = alive >> i & 1 ? order_key(c[i]) : 0;
   uint32_t best = 0;
   int at = 0x7fffffff;
   auto find_best = [&] {
-    best = 0;
-    at = 0x7fffffff;
+    best = keys[0];
+    at = lane;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const uint32_t key = order_key(c[i]);
-      if ((alive >> i & 1) && key > best) { best = key; at = lane + 32 * i; }
-    }
+    for (int i = 1; i < V; ++i)
+      if (keys[i] > best) { best = keys[i]; at = lane + 32 * i; }
   };
   find_best();
-  int mine = 0;
+  // Lane r gets the r-th candidate.  By score there is at least one more than k, and more as long as the last two
+  // are too close to tell apart (up to the warp's 32).
+  int mine = 0, found = 0;
   float last = 0.0f;
-  const int rounds = by_logit ? p.k : p.k + 1;   // one more round shows how near the first unchosen one is
-  for (int r = 0; r < rounds; ++r) {
+  bool close = false;
+  for (;; ++found) {
+    if (by_logit && found == p.k) break;
     const uint32_t key = __reduce_max_sync(kAll, best);
-    if (key == 0) break;                         // every expert is taken (the extra round)
+    if (key == 0) break;                         // every expert is taken
     const int e = __reduce_min_sync(kAll, best == key ? at : 0x7fffffff);
     if (!by_logit) {
       const float now = key_value(key);
-      if (r > 0 && last - now <= 2.0f * error + 0x1p-23f * fmaxf(fabsf(last), fabsf(now))) unsure = true;
+      const bool near = found > 0 && last - now <= 2.0f * error + 0x1p-23f * fmaxf(fabsf(last), fabsf(now));
+      if (found >= p.k && !near) break;          // the chosen ones are known, and no later one is near
+      close |= near;
       last = now;
+      if (found == 32) { unsure = true; break; }
     }
-    if (lane == r && r < p.k) mine = e;
+    if (lane == found) mine = e;
     if (lane == (e & 31)) {
-      alive &= ~(1u << (e >> 5));
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (lane + 32 * i == e) keys[i] = 0;
       find_best();
     }
   }
-  if (unsure) mine = choose_exactly<V>(p, row, lane, shared_row);   // (the same for the whole warp)
+  if (unsure) {                                  // (the same for the whole warp, as everything that follows)
+    mine = choose_exactly<V>(p, row, lane, shared_row);
+  } else if (close) {
+    // the candidates' scores again, in 64 bits, one a lane; each candidate's place is the number that come before it
+    double sum64 = 1.0;
+    if (softmax) {
+      double part = 0.0;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (v[i] != -INFINITY) part += exp(static_cast<double>(v[i]) - static_cast<double>(top));
+      sum64 = warp_sum<double>(part);
+    }
+    double exact = -INFINITY;
+    if (lane < found) {
+      const double l = static_cast<double>(logit_at(p, row + mine));
+      if (l != -INFINITY) {
+        exact = raw_score<double>(l, static_cast<double>(top), p.score);
+        if (softmax) exact /= sum64;
+        exact += static_cast<double>(sane(__ldg(p.bias + mine)));
+      }
+    }
+    int place = 0;
+    for (int j = 0; j < found; ++j) {
+      const double o = __shfl_sync(kAll, exact, j);
+      const int e = __shfl_sync(kAll, mine, j);
+      place += o > exact || (o == exact && e < mine);
+    }
+    if (lane >= found) place = 32;
+    int sorted = 0;
+    for (int j = 0; j < found; ++j) {
+      const int to = __shfl_sync(kAll, place, j), e = __shfl_sync(kAll, mine, j);
+      if (to == lane) sorted = e;
+    }
+    mine = sorted;
+  }
   const float l = lane < p.k ? logit_at(p, row + mine) : -INFINITY;
   // (shares among the chosen do not depend on the largest of all, which may be far above theirs)
   float s = raw_score<float>(l, p.renormalize ? warp_max<float>(l) : top, p.score);
@@ -307,8 +355,9 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
 }
 
 template <int V>
-__global__ void __launch_bounds__(256) select_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(256) select_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ __align__(16) unsigned char s_raw[];
+  launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.x * 8 + warp;
   if (token < p.S) select_token<V>(p, token, lane, reinterpret_cast<double*>(s_raw) + static_cast<size_t>(warp) * p.E);
@@ -316,28 +365,35 @@ __global__ void __launch_bounds__(256) select_kernel(const SelectParams p) {
 
 // ---- ordering ---------------------------------------------------------------------------------------
 
-constexpr int kOrderThreads = 512, kOrderWarps = kOrderThreads / 32, kOrderCtas = 8;
+constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32, kOrderCtas = 8;
+constexpr int kAhead = 8;   // pairs a lane loads before it uses the first
 
 // Stable counting sort of the pairs by expert: the CTAs of one cluster take consecutive runs of pairs, their
 // warps consecutive runs of those.  Pass one counts, pass two hands out places in the same order.
 // A token's experts differ, so pairs in order are tokens in order within an expert.
-__global__ void __launch_bounds__(kOrderThreads) order_kernel(const SelectParams p) {
-  extern __shared__ __align__(16) unsigned char s_raw[];
+__device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, int ctas, int cta, bool dependent) {
   const int E = p.E, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int* hist = reinterpret_cast<int*>(s_raw);      // [warps][E]: counts, then places already handed out
+  // hist [warps][E]: counts, then places already handed out
   int* total = hist + kOrderWarps * E;            // [E]: this CTA's pairs
   int* start = total + E;                         // [E]: first row of the expert, then of this CTA's share
   int* before = start + E;                        // [E]: this CTA's first slot within the expert
-  const int ctas = gridDim.x, cta = blockIdx.x;   // the grid is one cluster
   for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) hist[i] = 0;
   __syncthreads();
+  if (dependent) wait_for_primary();              // the ids are another grid's
   const long long pairs = static_cast<long long>(p.S) * p.k;
   const long long workers = static_cast<long long>(ctas) * kOrderWarps;
   const long long share = ((pairs + workers - 1) / workers + 31) & ~31ll;
   const long long first = min(pairs, (static_cast<long long>(cta) * kOrderWarps + warp) * share);
   const long long end = min(pairs, first + share);
   int* mine = hist + warp * E;
-  for (long long i = first + lane; i < end; i += 32) atomicAdd(mine + __ldg(p.ids + i), 1);
+  for (long long i0 = first; i0 < end; i0 += 32 * kAhead) {
+    int e[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) e[j] = i0 + 32 * j + lane < end ? p.ids[i0 + 32 * j + lane] : -1;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (e[j] >= 0) atomicAdd(mine + e[j], 1);
+  }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kOrderThreads) {
     int sum = 0;
@@ -383,23 +439,30 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const SelectParams
   }
   __syncthreads();
   if (p.positions != nullptr || p.table != nullptr) {
-    for (long long i0 = first; i0 < end; i0 += 32) {
-      const long long i = i0 + lane;
-      const int e = i < end ? __ldg(p.ids + i) : -1;
-      const unsigned same = __match_any_sync(kAll, e);
-      const int rank = __popc(same & ((1u << lane) - 1));
-      int slot = 0;
-      if (e >= 0) slot = before[e] + mine[e] + rank;
-      __syncwarp();
-      if (e >= 0 && rank == 0) mine[e] += __popc(same);
-      __syncwarp();
-      if (e >= 0) {
-        if (p.positions != nullptr) p.positions[i] = start[e] + slot;
-        if (p.table != nullptr) {
-          const float w = __ldg(p.weights + i);
-          if (slot < p.capacity)
-            p.table[static_cast<size_t>(e) * p.round_ec + slot] = TokenSlot{static_cast<uint32_t>(i / p.k), w};
-          p.routes[i] = Route{e, slot, w, 0};
+    for (long long i0 = first; i0 < end; i0 += 32 * kAhead) {
+      int ids[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) ids[j] = i0 + 32 * j + lane < end ? p.ids[i0 + 32 * j + lane] : -1;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const long long i = i0 + 32 * j + lane;
+        const int e = ids[j];
+        if (i0 + 32 * j >= end) break;
+        const unsigned same = __match_any_sync(kAll, e);
+        const int rank = __popc(same & ((1u << lane) - 1));
+        int slot = 0;
+        if (e >= 0) slot = before[e] + mine[e] + rank;
+        __syncwarp();
+        if (e >= 0 && rank == 0) mine[e] += __popc(same);
+        __syncwarp();
+        if (e >= 0) {
+          if (p.positions != nullptr) p.positions[i] = start[e] + slot;
+          if (p.table != nullptr) {
+            const float w = p.weights[i];
+            if (slot < p.capacity)
+              p.table[static_cast<size_t>(e) * p.round_ec + slot] = TokenSlot{static_cast<uint32_t>(i / p.k), w};
+            p.routes[i] = Route{e, slot, w, 0};
+          }
         }
       }
     }
@@ -407,45 +470,76 @@ __global__ void __launch_bounds__(kOrderThreads) order_kernel(const SelectParams
   if (ctas > 1) ptx::cluster_sync_all();   // no CTA leaves while another reads its totals
 }
 
+__global__ void __launch_bounds__(kOrderThreads) order_kernel(const __grid_constant__ SelectParams p) {
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  order_pairs(p, reinterpret_cast<int*>(s_raw), gridDim.x, blockIdx.x, p.S > 0);   // (the grid is one cluster)
+}
+
+// Few tokens: one CTA chooses and orders.
+template <int V>
+__global__ void __launch_bounds__(kOrderThreads) select_few_kernel(const __grid_constant__ SelectParams p) {
+  extern __shared__ __align__(16) unsigned char s_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int token = warp; token < p.S; token += kOrderWarps)
+    select_token<V>(p, token, lane, reinterpret_cast<double*>(s_raw) + static_cast<size_t>(warp) * p.E);
+  __syncthreads();
+  order_pairs(p, reinterpret_cast<int*>(s_raw), 1, 0, false);
+}
+
 size_t order_smem(int E) { return static_cast<size_t>(kOrderWarps + 3) * E * sizeof(int); }
 
-cudaError_t launch_order(const SelectParams& p, cudaStream_t stream) {
-  const size_t smem = order_smem(p.E);
+template <typename Kernel>
+cudaError_t launch(Kernel kernel, const SelectParams& p, int grid, int threads, size_t smem, int cluster, bool dependent,
+                   cudaStream_t stream) {
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
   }
-  const long long pairs = static_cast<long long>(p.S) * p.k;
-  const int ctas = pairs <= 4 * kOrderThreads ? 1 : kOrderCtas;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kOrderThreads);
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (dependent) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = n;
   ++g_launches;
-  return cudaLaunchKernelEx(&cfg, order_kernel, p);
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
+
+// Up to this many tokens one CTA does it all: two rounds of its 32 warps (64 tokens of 256 experts by one launch and
+// by two: see the figures at the top of the file).
+constexpr int kFewTokens = 64;
 
 template <int V>
 cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
-  if (p.S > 0) {
-    const size_t smem = p.groups > 1 ? 8 * static_cast<size_t>(p.E) * sizeof(double) : 0;
-    if (smem > 48 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(select_kernel<V>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-      if (e != cudaSuccess) return e;
+  const size_t group_row = p.groups > 1 ? static_cast<size_t>(p.E) * sizeof(double) : 0;
+  const size_t order = order_smem(p.E);
+  if constexpr (V <= 8) {   // (the registers of 32 warps)
+    if (p.S <= kFewTokens) {
+      const size_t rows = kOrderWarps * group_row;
+      return launch(select_few_kernel<V>, p, 1, kOrderThreads, rows > order ? rows : order, 1, false, stream);
     }
-    select_kernel<V><<<(p.S + 7) / 8, 256, smem, stream>>>(p);
-    ++g_launches;
-    const cudaError_t e = cudaGetLastError();
+  }
+  if (p.S > 0) {
+    const cudaError_t e = launch(select_kernel<V>, p, (p.S + 7) / 8, 256, 8 * group_row, 1, false, stream);
     if (e != cudaSuccess) return e;
   }
-  return launch_order(p, stream);
+  const long long pairs = static_cast<long long>(p.S) * p.k;
+  const int ctas = pairs <= kOrderThreads ? 1 : kOrderCtas;
+  return launch(order_kernel, p, ctas, kOrderThreads, order, ctas, p.S > 0, stream);
 }
 
 int check(const fmoe_select_args* a) {
