@@ -211,16 +211,19 @@ __device__ __noinline__ int choose_exactly(const SelectParams& p, size_t row, in
 template <int V>
 __device__ __forceinline__ void select_token(const SelectParams& p, int token, int lane, double* shared_row) {
   const size_t row = static_cast<size_t>(token) * p.E;
+  const bool softmax = p.score == FMOE_SCORE_SOFTMAX, by_score = p.bias != nullptr || p.groups > 1;
   float v[V];
-  float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int e = lane + 32 * i;
     v[i] = e < p.E ? logit_at(p, row + e) : -INFINITY;
-    top = fmaxf(top, v[i]);
   }
-  top = warp_max<float>(top);
-  const bool softmax = p.score == FMOE_SCORE_SOFTMAX, by_score = p.bias != nullptr || p.groups > 1;
+  float top = -INFINITY;
+  if (softmax && (by_score || !p.renormalize)) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = fmaxf(top, v[i]);
+    top = warp_max<float>(top);
+  }
   float sum = 1.0f;
   float c[V];   // what is compared
   if (by_score || (softmax && !p.renormalize)) {
@@ -266,19 +269,25 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
     for (int i = 0; i < V; ++i) c[i] = v[i];
   }
   const uint32_t alive = alive_bits<V>(p.E, p.groups, kept, lane);
-  uint32_t keys[V];   // 0: not there, or taken
+  // this lane's candidates, best first (equal ones in index order); 0: none left
+  uint32_t keys[V];
+  int at[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) keys[i] = alive >> i & 1 ? order_key(c[i]) : 0;
-  uint32_t best = 0;
-  int at = 0x7fffffff;
-  auto find_best = [&] {
-    best = keys[0];
-    at = lane;
+  for (int i = 0; i < V; ++i) {
+    keys[i] = alive >> i & 1 ? order_key(c[i]) : 0;
+    at[i] = lane + 32 * i;
+  }
+  // odd-even transposition: neighbours only, so equal keys keep their order
 #pragma unroll
-    for (int i = 1; i < V; ++i)
-      if (keys[i] > best) { best = keys[i]; at = lane + 32 * i; }
-  };
-  find_best();
+  for (int pass = 0; pass < V; ++pass)
+#pragma unroll
+    for (int i = pass & 1; i + 1 < V; i += 2) {
+      const bool swap = keys[i + 1] > keys[i];
+      const uint32_t hi = swap ? keys[i + 1] : keys[i], lo = swap ? keys[i] : keys[i + 1];
+      const int first = swap ? at[i + 1] : at[i], then = swap ? at[i] : at[i + 1];
+      keys[i] = hi; keys[i + 1] = lo;
+      at[i] = first; at[i + 1] = then;
+    }
   // Lane r gets the r-th candidate.  By score there is at least one more than k, and more as long as the last two
   // are too close to tell apart (up to the warp's 32).
   int mine = 0, found = 0;
@@ -286,9 +295,9 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
   bool close = false;
   for (;; ++found) {
     if (by_logit && found == p.k) break;
-    const uint32_t key = __reduce_max_sync(kAll, best);
+    const uint32_t key = __reduce_max_sync(kAll, keys[0]);
     if (key == 0) break;                         // every expert is taken
-    const int e = __reduce_min_sync(kAll, best == key ? at : 0x7fffffff);
+    const int e = __reduce_min_sync(kAll, keys[0] == key ? at[0] : 0x7fffffff);
     if (!by_logit) {
       const float now = key_value(key);
       const bool near = found > 0 && last - now <= 2.0f * error + 0x1p-23f * fmaxf(fabsf(last), fabsf(now));
@@ -298,12 +307,13 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
       if (found == 32) { unsure = true; break; }
     }
     if (lane == found) mine = e;
-    if (lane == (e & 31)) {
+    const bool took = lane == (e & 31);
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (lane + 32 * i == e) keys[i] = 0;
-      find_best();
+    for (int i = 0; i + 1 < V; ++i) {
+      keys[i] = took ? keys[i + 1] : keys[i];
+      at[i] = took ? at[i + 1] : at[i];
     }
+    keys[V - 1] = took ? 0 : keys[V - 1];
   }
   if (unsure) {                                  // (the same for the whole warp, as everything that follows)
     mine = choose_exactly<V>(p, row, lane, shared_row);
@@ -342,7 +352,7 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
   }
   const float l = lane < p.k ? logit_at(p, row + mine) : -INFINITY;
   // (shares among the chosen do not depend on the largest of all, which may be far above theirs)
-  float s = raw_score<float>(l, p.renormalize ? warp_max<float>(l) : top, p.score);
+  float s = raw_score<float>(l, p.renormalize ? (by_logit ? __shfl_sync(kAll, l, 0) : warp_max<float>(l)) : top, p.score);
   if (softmax && !p.renormalize && sum > 0.0f) s = s / sum;
   if (p.renormalize) {
     const float total = warp_sum<float>(s);
@@ -368,111 +378,149 @@ __global__ void __launch_bounds__(256) select_kernel(const __grid_constant__ Sel
 constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32, kOrderCtas = 8;
 constexpr int kAhead = 8;   // pairs a lane loads before it uses the first
 
-// Stable counting sort of the pairs by expert: the CTAs of one cluster take consecutive runs of pairs, their
-// warps consecutive runs of those.  Pass one counts, pass two hands out places in the same order.
-// A token's experts differ, so pairs in order are tokens in order within an expert.
-__device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, int ctas, int cta, bool dependent) {
+// What is known of pair i: its expert e, its slot there, and the first row of the expert.
+__device__ __forceinline__ void place_pair(const SelectParams& p, long long i, int e, int slot, int first_row) {
+  if (p.positions != nullptr) p.positions[i] = first_row + slot;
+  if (p.table != nullptr) {
+    const float w = p.weights[i];
+    if (slot < p.capacity)
+      p.table[static_cast<size_t>(e) * p.round_ec + slot] = TokenSlot{static_cast<uint32_t>(i / p.k), w};
+    p.routes[i] = Route{e, slot, w, 0};
+  }
+}
+
+// The lanes whose id is this lane's, by one ballot for each of the ids' bits (match.any takes about 1000 cycles for 32
+// ids that differ).  id < 0: none.
+__device__ __forceinline__ unsigned lanes_alike(int id, int bits) {
+  const unsigned here = __ballot_sync(kAll, id >= 0);
+  unsigned same = id >= 0 ? here : 0;
+#pragma unroll
+  for (int b = 0; b < 10; ++b) {
+    if (b < bits) {
+      const bool one = id >> b & 1;
+      const unsigned ones = __ballot_sync(kAll, one);
+      same &= one ? ones : ~ones;
+    }
+  }
+  return same;
+}
+
+// Stable counting sort of the pairs by expert: the CTAs of one cluster (or one CTA) take consecutive runs of pairs,
+// their warps consecutive runs of those.  Pass one counts, pass two hands out places in the same order; in between
+// the CTAs' counts meet in distributed shared memory.  (A token's experts differ, so pairs in order are tokens in
+// order within an expert.)  What it costs is its chain of steps, so each step has its loads in flight together.
+// One CTA per expert that scans all pairs for itself needs no steps but reads the pairs once per expert: 65536 pairs
+// of 128 experts took 18 us.
+template <int kCtas>
+__device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bool dependent) {
+  __shared__ int s_sum[kOrderWarps];
   const int E = p.E, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = kCtas > 1 ? blockIdx.x : 0;     // (the grid is one cluster)
   // hist [warps][E]: counts, then places already handed out
   int* total = hist + kOrderWarps * E;            // [E]: this CTA's pairs
-  int* start = total + E;                         // [E]: first row of the expert, then of this CTA's share
-  int* before = start + E;                        // [E]: this CTA's first slot within the expert
   for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) hist[i] = 0;
   __syncthreads();
   if (dependent) wait_for_primary();              // the ids are another grid's
   const long long pairs = static_cast<long long>(p.S) * p.k;
-  const long long workers = static_cast<long long>(ctas) * kOrderWarps;
-  const long long share = ((pairs + workers - 1) / workers + 31) & ~31ll;
+  constexpr long long kWorkers = static_cast<long long>(kCtas) * kOrderWarps;
+  const long long share = ((pairs + kWorkers - 1) / kWorkers + 31) & ~31ll;
   const long long first = min(pairs, (static_cast<long long>(cta) * kOrderWarps + warp) * share);
-  const long long end = min(pairs, first + share);
+  const int n = static_cast<int>(min(pairs, first + share) - first);
+  const int32_t* ids = p.ids + first;
   int* mine = hist + warp * E;
-  for (long long i0 = first; i0 < end; i0 += 32 * kAhead) {
-    int e[kAhead];
+  int ahead[kAhead];
+  auto load = [&](int i0) {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) e[j] = i0 + 32 * j + lane < end ? p.ids[i0 + 32 * j + lane] : -1;
+    for (int j = 0; j < kAhead; ++j) ahead[j] = i0 + 32 * j + lane < n ? ids[i0 + 32 * j + lane] : -1;
+  };
+  for (int i0 = 0; i0 < n; i0 += 32 * kAhead) {
+    load(i0);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-      if (e[j] >= 0) atomicAdd(mine + e[j], 1);
+      if (ahead[j] >= 0) atomicAdd(mine + ahead[j], 1);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kOrderThreads) {
-    int sum = 0;
+  const int e = threadIdx.x;                      // (at most kOrderThreads experts)
+  if (e < E) {
+    int c[kOrderWarps], sum = 0;
+#pragma unroll
+    for (int w = 0; w < kOrderWarps; ++w) c[w] = hist[w * E + e];
+#pragma unroll
     for (int w = 0; w < kOrderWarps; ++w) {
-      const int c = hist[w * E + e];
       hist[w * E + e] = sum;
-      sum += c;
+      sum += c[w];
     }
     total[e] = sum;
   }
-  if (ctas > 1) ptx::cluster_sync_all(); else __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kOrderThreads) {
-    int all = 0, lower = 0;
-    for (int c = 0; c < ctas; ++c) {
-      int n;
-      if (ctas > 1) asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(n) : "r"(ptx::map_to_cta(total + e, c)) : "memory");
-      else n = total[e];
-      if (c < cta) lower += n;
-      all += n;
+  int all = 0, lower = 0;                         // expert e's pairs: of all CTAs, of the CTAs before this one
+  if constexpr (kCtas > 1) {
+    ptx::cluster_sync_all();
+    if (e < E) {
+      int c[kCtas];
+#pragma unroll
+      for (int q = 0; q < kCtas; ++q)
+        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c[q]) : "r"(ptx::map_to_cta(total + e, q)) : "memory");
+#pragma unroll
+      for (int q = 0; q < kCtas; ++q) {
+        lower += q < cta ? c[q] : 0;
+        all += c[q];
+      }
     }
-    before[e] = lower;
-    start[e] = all;
-    if (cta == 0) p.counts[e] = all;
+  } else if (e < E) {
+    all = total[e];
+  }
+  // exclusive sum over the experts
+  int sum = all;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(kAll, sum, d);
+    if (lane >= d) sum += o;
+  }
+  if (lane == 31) s_sum[warp] = sum;
+  __syncthreads();
+  int before = lane < warp ? s_sum[lane] : 0;
+  before = __reduce_add_sync(kAll, before);
+  const int start = before + sum - all;
+  if constexpr (kCtas > 1) ptx::cluster_sync_all();   // every total has been read
+  if (e < E) {
+    total[e] = start;                             // from here on: the expert's first row
+    if (lower != 0) {
+#pragma unroll
+      for (int w = 0; w < kOrderWarps; ++w) hist[w * E + e] += lower;
+    }
+    if (cta == 0) {
+      p.counts[e] = all;
+      if (p.offsets != nullptr) {
+        p.offsets[e] = start;
+        if (e == E - 1) p.offsets[E] = start + all;
+      }
+    }
   }
   __syncthreads();
-  if (warp == 0) {   // exclusive sum over the experts
-    int carry = 0;
-    for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + lane, own = e < E ? start[e] : 0;
-      int sum = own;
+  if (p.positions == nullptr && p.table == nullptr) return;
+  const bool once = n <= 32 * kAhead;             // the ids are still in registers
+  const int id_bits = 32 - __clz(E - 1);          // (E = 1: no bits)
+  for (int i0 = 0; i0 < n; i0 += 32 * kAhead) {
+    if (!once) load(i0);
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(kAll, sum, d);
-        if (lane >= d) sum += o;
-      }
-      if (e < E) {
-        start[e] = carry + sum - own;
-        if (cta == 0 && p.offsets != nullptr) p.offsets[e] = carry + sum - own;
-      }
-      carry += __shfl_sync(kAll, sum, 31);
-    }
-    if (cta == 0 && lane == 0 && p.offsets != nullptr) p.offsets[E] = carry;
-  }
-  __syncthreads();
-  if (p.positions != nullptr || p.table != nullptr) {
-    for (long long i0 = first; i0 < end; i0 += 32 * kAhead) {
-      int ids[kAhead];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) ids[j] = i0 + 32 * j + lane < end ? p.ids[i0 + 32 * j + lane] : -1;
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const long long i = i0 + 32 * j + lane;
-        const int e = ids[j];
-        if (i0 + 32 * j >= end) break;
-        const unsigned same = __match_any_sync(kAll, e);
-        const int rank = __popc(same & ((1u << lane) - 1));
-        int slot = 0;
-        if (e >= 0) slot = before[e] + mine[e] + rank;
-        __syncwarp();
-        if (e >= 0 && rank == 0) mine[e] += __popc(same);
-        __syncwarp();
-        if (e >= 0) {
-          if (p.positions != nullptr) p.positions[i] = start[e] + slot;
-          if (p.table != nullptr) {
-            const float w = p.weights[i];
-            if (slot < p.capacity)
-              p.table[static_cast<size_t>(e) * p.round_ec + slot] = TokenSlot{static_cast<uint32_t>(i / p.k), w};
-            p.routes[i] = Route{e, slot, w, 0};
-          }
-        }
-      }
+    for (int j = 0; j < kAhead; ++j) {
+      if (i0 + 32 * j >= n) break;
+      const int id = ahead[j];
+      const unsigned same = lanes_alike(id, id_bits);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      const int slot = id >= 0 ? mine[id] + rank : 0;
+      __syncwarp();
+      if (id >= 0 && rank == 0) mine[id] += __popc(same);
+      __syncwarp();
+      if (id >= 0) place_pair(p, first + i0 + 32 * j + lane, id, slot, total[id]);
     }
   }
-  if (ctas > 1) ptx::cluster_sync_all();   // no CTA leaves while another reads its totals
 }
 
 __global__ void __launch_bounds__(kOrderThreads) order_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ __align__(16) unsigned char s_raw[];
-  order_pairs(p, reinterpret_cast<int*>(s_raw), gridDim.x, blockIdx.x, p.S > 0);   // (the grid is one cluster)
+  if (gridDim.x == 1) order_pairs<1>(p, reinterpret_cast<int*>(s_raw), p.S > 0);
+  else order_pairs<kOrderCtas>(p, reinterpret_cast<int*>(s_raw), p.S > 0);
 }
 
 // Few tokens: one CTA chooses and orders.
@@ -483,10 +531,8 @@ __global__ void __launch_bounds__(kOrderThreads) select_few_kernel(const __grid_
   for (int token = warp; token < p.S; token += kOrderWarps)
     select_token<V>(p, token, lane, reinterpret_cast<double*>(s_raw) + static_cast<size_t>(warp) * p.E);
   __syncthreads();
-  order_pairs(p, reinterpret_cast<int*>(s_raw), 1, 0, false);
+  order_pairs<1>(p, reinterpret_cast<int*>(s_raw), false);
 }
-
-size_t order_smem(int E) { return static_cast<size_t>(kOrderWarps + 3) * E * sizeof(int); }
 
 template <typename Kernel>
 cudaError_t launch(Kernel kernel, const SelectParams& p, int grid, int threads, size_t smem, int cluster, bool dependent,
@@ -519,14 +565,13 @@ cudaError_t launch(Kernel kernel, const SelectParams& p, int grid, int threads, 
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-// Up to this many tokens one CTA does it all: two rounds of its 32 warps (64 tokens of 256 experts by one launch and
-// by two: see the figures at the top of the file).
+// Up to this many tokens one CTA does it all, in two rounds of its 32 warps.
 constexpr int kFewTokens = 64;
 
 template <int V>
 cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
   const size_t group_row = p.groups > 1 ? static_cast<size_t>(p.E) * sizeof(double) : 0;
-  const size_t order = order_smem(p.E);
+  const size_t order = static_cast<size_t>(kOrderWarps + 1) * p.E * sizeof(int);
   if constexpr (V <= 8) {   // (the registers of 32 warps)
     if (p.S <= kFewTokens) {
       const size_t rows = kOrderWarps * group_row;
@@ -537,8 +582,7 @@ cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
     const cudaError_t e = launch(select_kernel<V>, p, (p.S + 7) / 8, 256, 8 * group_row, 1, false, stream);
     if (e != cudaSuccess) return e;
   }
-  const long long pairs = static_cast<long long>(p.S) * p.k;
-  const int ctas = pairs <= kOrderThreads ? 1 : kOrderCtas;
+  const int ctas = static_cast<long long>(p.S) * p.k <= kOrderThreads ? 1 : kOrderCtas;
   return launch(order_kernel, p, ctas, kOrderThreads, order, ctas, p.S > 0, stream);
 }
 
