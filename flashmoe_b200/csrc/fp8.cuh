@@ -193,6 +193,12 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64
       ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// ---- programmatic launches ------------------------------------------------------------------------
+// The next grid may start when every CTA of this one has said so, and waits for this one's
+// results where it needs them.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- host side -----------------------------------------------------------------------------------
 // Makes `device` current for the scope and puts the caller's device back.
 struct OnDevice {
@@ -211,6 +217,10 @@ struct OnDevice {
   OnDevice& operator=(const OnDevice&) = delete;
 };
 inline bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+// The products, launched under the tail of the stream's last kernel where `dependent`: that kernel must have been
+// launched after everything but A was complete, and write A.
+int matmul(const fmoe_fp8_matmul_args* a, bool dependent, cudaStream_t stream);
+int gated_matmul(const fmoe_fp8_gated_args* a, bool dependent, cudaStream_t stream);
 inline int element_bytes(int data_type) { return data_type == FMOE_DT_FP32 ? 4 : 2; }
 
 }  // namespace fmoe::fp8

@@ -1,5 +1,9 @@
 // The expert layer on 8-bit weights as a chain of four launches: quantise the tokens into expert
 // order, gated up product (activation and quantisation in its epilogue), down product, weighted sum.
+// Each but the first is launched under the tail of the one before: it sets up, and the few-row products fetch their
+// first weights, before it waits for what that one writes.  The first is an ordinary launch, so whatever the chain
+// reads from outside is complete by then; every CTA of every kernel waits before it ends, so the end of the last one
+// is the end of all.
 #include "fp8.cuh"
 
 namespace fmoe::fp8 {
@@ -18,6 +22,7 @@ struct CombineParams {
 // out[t] = sum over j of weights[t, j] * y[positions[t, j]], in fp32 in the order of j; eight values a thread.
 template <typename T>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
+  wait_for_primary();   // the down product's rows
   const int vectors = p.dim >> 3;
   const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   const long long token = i / vectors;
@@ -41,9 +46,17 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
 template <typename T>
 cudaError_t launch_combine(const CombineParams& p, cudaStream_t stream) {
   const long long threads = static_cast<long long>(p.tokens) * (p.dim >> 3);
-  combine_kernel<T><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, stream>>>(p);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((threads + 255) / 256));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   ++g_launches;
-  return cudaGetLastError();
+  return cudaLaunchKernelEx(&cfg, combine_kernel<T>, p);
 }
 
 // Parts of the workspace, each 256-byte aligned.
@@ -124,8 +137,8 @@ int fmoe_fp8_experts(const fmoe_fp8_experts_args* a, void* stream) {
   const fmoe_fp8_matmul_args down{ws + pl.hq, reinterpret_cast<float*>(ws + pl.hs), a->down, a->down_scale, ws + pl.y, a->offsets,
                                   pairs, a->token_dim, a->ffn_size, a->num_experts, a->data_type, a->device_id};
   rc = fmoe_fp8_quantize(&quantize, stream);
-  if (rc == FMOE_OK) rc = fmoe_fp8_gated_matmul(&gated, stream);
-  if (rc == FMOE_OK) rc = fmoe_fp8_matmul(&down, stream);
+  if (rc == FMOE_OK) rc = gated_matmul(&gated, true, static_cast<cudaStream_t>(stream));
+  if (rc == FMOE_OK) rc = matmul(&down, true, static_cast<cudaStream_t>(stream));
   if (rc != FMOE_OK) return rc;
   OnDevice on(a->device_id);
   if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));

@@ -51,6 +51,7 @@ struct ProductParams {
   float* out_scale;            // gated form
   int act, has_v;              // gated form
   int wide;                    // output rows may be stored 32 bytes at a time
+  int dependent;               // launched under the tail of the kernel that writes A (weights and offsets are older)
   long long spin_limit;
 };
 
@@ -299,6 +300,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   tc_fence_after_sync();
   const uint32_t tmem = sh.tmem_base;
   const bool second = !kGated || p.has_v != 0;   // whether the second 128 weight rows exist
+  launch_dependents();
+  if (p.dependent) wait_for_primary();
 
   if (warp < kEpilogueWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
@@ -659,12 +662,30 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
   tc_fence_after_sync();
   const uint32_t tmem = sh.tmem_base;
   const bool second = kGated && p.has_v != 0;
+  launch_dependents();
+  if (p.dependent && warp != 0) wait_for_primary();
 
   if (warp == 0) {
     const uint32_t bytes = N::kRowBytes + (second ? 2 : 1) * kBoxBytes;
     uint32_t stage = 0, phase = 1;
     Tile t;
     bool ok = true;
+    int early = 0;   // blocks whose weights are on their way before the rows exist
+    if (p.dependent) {
+      if (find_tile(sh.table, p, first_tile, kRows, kBlock, t)) {
+        early = min(kStages, kb1 - kb0);
+        if (elect_one()) {
+          for (int j = 0; j < early; ++j) {
+            unsigned char* to = ring + j * N::kStageBytes;
+            mbar_expect_tx(&sh.full[j], bytes);
+            tma_load_2d(to, &map_w0, &sh.full[j], (kb0 + j) * kBlock, t.expert * p.n + t.n0);
+            if (second) tma_load_2d(to + kBoxBytes, &map_w1, &sh.full[j], (kb0 + j) * kBlock, t.expert * p.n + t.n0);
+          }
+        }
+        __syncwarp();
+      }
+      wait_for_primary();
+    }
     for (int i = first_tile; ok && find_tile(sh.table, p, i, kRows, kBlock, t); i += tile_step) {
       const int w_row = t.expert * p.n + t.n0;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -672,12 +693,15 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         if (!ok) break;
         if (elect_one()) {
           unsigned char* to = ring + stage * N::kStageBytes;
-          mbar_expect_tx(&sh.full[stage], bytes);
-          tma_load_2d(to, &map_w0, &sh.full[stage], kb * kBlock, w_row);
-          if (second) tma_load_2d(to + kBoxBytes, &map_w1, &sh.full[stage], kb * kBlock, w_row);
+          if (early <= 0) {
+            mbar_expect_tx(&sh.full[stage], bytes);
+            tma_load_2d(to, &map_w0, &sh.full[stage], kb * kBlock, w_row);
+            if (second) tma_load_2d(to + kBoxBytes, &map_w1, &sh.full[stage], kb * kBlock, w_row);
+          }
           tma_load_2d(to + N::kWeights * kBoxBytes, &map_a, &sh.full[stage], kb * kBlock, t.row0);
         }
         __syncwarp();
+        --early;
         if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
       if (!ok && lane == 0) wait_failed(&sh.abort_word, FMOE_PHASE_PIPE_EMPTY, i);
@@ -964,12 +988,21 @@ int launch_kernel(Kernel kernel, std::atomic<unsigned long long>& prepared, size
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (p.dependent) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cfg.numAttrs = n;
   e = cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], p);
   ++g_launches;
   if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("8-bit product launch: ") + cudaGetErrorString(e));
@@ -1097,14 +1130,7 @@ ProductParams product_params(int m, int n, int k, int experts, const int32_t* of
 
 }  // namespace
 
-}  // namespace fmoe::fp8
-
-using namespace fmoe;
-using namespace fmoe::fp8;
-
-extern "C" {
-
-int fmoe_fp8_matmul(const fmoe_fp8_matmul_args* a, void* stream) {
+int matmul(const fmoe_fp8_matmul_args* a, bool dependent, cudaStream_t st) {
   if (a == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "arguments are null");
   int rc = check_product(a->a, a->a_scale, a->w, a->w_scale, a->offsets, a->m, a->n, a->k, a->num_experts, a->device_id);
   if (rc != FMOE_OK) return rc;
@@ -1121,13 +1147,13 @@ int fmoe_fp8_matmul(const fmoe_fp8_matmul_args* a, void* stream) {
   p.w_scale[0] = a->w_scale;
   p.out = a->out;
   p.wide = !misaligned(a->out, 32) && (static_cast<size_t>(a->n) * eb) % 32 == 0;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  p.dependent = dependent;
   if (a->data_type == FMOE_DT_BF16) return launch_product<__nv_bfloat16>(p, a->a, a->w, a->w, a->device_id, st);
   if (a->data_type == FMOE_DT_FP16) return launch_product<__half>(p, a->a, a->w, a->w, a->device_id, st);
   return launch_product<float>(p, a->a, a->w, a->w, a->device_id, st);
 }
 
-int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* a, void* stream) {
+int gated_matmul(const fmoe_fp8_gated_args* a, bool dependent, cudaStream_t st) {
   if (a == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "arguments are null");
   int rc = check_product(a->a, a->a_scale, a->up, a->up_scale, a->offsets, a->m, a->ffn_size, a->k, a->num_experts,
                          a->device_id);
@@ -1151,7 +1177,21 @@ int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* a, void* stream) {
   p.out_scale = a->scale;
   p.act = a->act_type;
   p.has_v = a->up_v != nullptr;
-  return launch_product<Codes>(p, a->a, a->up, a->up_v != nullptr ? a->up_v : a->up, a->device_id, static_cast<cudaStream_t>(stream));
+  p.dependent = dependent;
+  return launch_product<Codes>(p, a->a, a->up, a->up_v != nullptr ? a->up_v : a->up, a->device_id, st);
+}
+
+}  // namespace fmoe::fp8
+
+using namespace fmoe;
+using namespace fmoe::fp8;
+
+extern "C" {
+
+int fmoe_fp8_matmul(const fmoe_fp8_matmul_args* a, void* stream) { return matmul(a, false, static_cast<cudaStream_t>(stream)); }
+
+int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* a, void* stream) {
+  return gated_matmul(a, false, static_cast<cudaStream_t>(stream));
 }
 
 int fmoe_fp8_last_status(int32_t device_id, void* stream, fmoe_status* out) {

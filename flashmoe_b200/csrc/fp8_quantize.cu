@@ -74,6 +74,7 @@ struct Raw16 {
 // Eight threads a block of 128, sixteen values each.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams p) {
+  launch_dependents();   // (of the expert layer: its next kernel)
   const uint32_t block = blockIdx.x * (256 / 8) + (threadIdx.x >> 3);   // (the host sees to it that it fits)
   const int sub = threadIdx.x & 7;
   const uint32_t row32 = block / static_cast<uint32_t>(p.col_blocks);

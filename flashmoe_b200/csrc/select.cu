@@ -37,11 +37,6 @@ struct SelectParams {
   float scale;
 };
 
-// Programmatic launches: the next grid may start when every CTA of this one has said so, and waits for this one's
-// results where it needs them.
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // ---- choosing ---------------------------------------------------------------------------------------
 
 // A masked expert (-infinity or NaN) orders below every other; +infinity is the largest finite number.
@@ -367,7 +362,7 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
 template <int V>
 __global__ void __launch_bounds__(256) select_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ __align__(16) unsigned char s_raw[];
-  launch_dependents();
+  fp8::launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.x * 8 + warp;
   if (token < p.S) select_token<V>(p, token, lane, reinterpret_cast<double*>(s_raw) + static_cast<size_t>(warp) * p.E);
@@ -420,7 +415,7 @@ __device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bo
   int* total = hist + kOrderWarps * E;            // [E]: this CTA's pairs
   for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) hist[i] = 0;
   __syncthreads();
-  if (dependent) wait_for_primary();              // the ids are another grid's
+  if (dependent) fp8::wait_for_primary();              // the ids are another grid's
   const long long pairs = static_cast<long long>(p.S) * p.k;
   constexpr long long kWorkers = static_cast<long long>(kCtas) * kOrderWarps;
   const long long share = ((pairs + kWorkers - 1) / kWorkers + 31) & ~31ll;
