@@ -144,25 +144,34 @@ __device__ __forceinline__ uint4 pack16(const float (&f)[16 / sizeof(T)]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// x sigmoid(x) within 2^-21 of its value: exp(-x) = 2^n 2^f with f = -x log2(e) - n kept to fp32 precision
-// (log2(e) in two parts), so that only the hardware's exponential (2^-22), the sum and the reciprocal
-// (2^-23) round.
+// x sigmoid(x) within 2^-21 of its value: exp(-x) = 2^t (1 + d ln 2) with t = -x log2(e) rounded and d what the
+// rounding and the second part of log2(e) left out, so that only the hardware's exponential (2^-22), the sum and
+// the reciprocal (2^-23) round.  Two special-function operations; a range reduction would take two more.
 __device__ __forceinline__ float silu(float x) {
-  const float y = fminf(fmaxf(-x, -87.0f), 87.0f);   // 2^n stays a normal number
-  const float n = rintf(y * 1.44269502e+00f);
-  const float f = fmaf(y, 1.92596303e-08f, fmaf(y, 1.44269502e+00f, -n));
+  const float t = x * -1.44269502e+00f;
+  const float d = fmaf(x, -1.92596303e-08f, fmaf(x, -1.44269502e+00f, -t));
   float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(f));
-  e = fmaf(e, __int_as_float((static_cast<int>(n) + 127) << 23), 1.0f);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(t, 126.0f)));
+  e = fmaf(e * 0.693147182f, d, e) + 1.0f;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e));
   return x < -87.0f ? 0.0f : x * r;   // (below -87 the value is above -2^-118)
 }
-__device__ __forceinline__ float activate(float x, int act) {
+template <int kAct>
+__device__ __forceinline__ float activate(float x) {
+  if constexpr (kAct == FMOE_ACT_SILU) return silu(x);
+  else if constexpr (kAct == FMOE_ACT_GELU) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+  else if constexpr (kAct == FMOE_ACT_RELU) return fmaxf(x, 0.0f);
+  else return x;
+}
+// f(the activation as a compile-time constant): a choice per value, unrolled over a tile, is four times the code,
+// and fetching it took a third of the tile's time
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
   switch (act) {
-    case FMOE_ACT_SILU: return silu(x);
-    case FMOE_ACT_GELU: return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
-    case FMOE_ACT_RELU: return fmaxf(x, 0.0f);
-    default: return x;
+    case FMOE_ACT_SILU: f(std::integral_constant<int, FMOE_ACT_SILU>{}); break;
+    case FMOE_ACT_GELU: f(std::integral_constant<int, FMOE_ACT_GELU>{}); break;
+    case FMOE_ACT_RELU: f(std::integral_constant<int, FMOE_ACT_RELU>{}); break;
+    default: f(std::integral_constant<int, FMOE_ACT_IDENTITY>{});
   }
 }
 

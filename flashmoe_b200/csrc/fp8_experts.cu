@@ -10,6 +10,7 @@ namespace fmoe::fp8 {
 namespace {
 
 constexpr int kMaxDevices = 64;
+constexpr int kCombineThreads = 128;
 
 struct CombineParams {
   const void* y;              // [tokens * top_k, dim], expert order
@@ -21,7 +22,7 @@ struct CombineParams {
 
 // out[t] = sum over j of weights[t, j] * y[positions[t, j]], in fp32 in the order of j; eight values a thread.
 template <typename T>
-__global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const CombineParams p) {
   wait_for_primary();   // the down product's rows
   const int vectors = p.dim >> 3;
   const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -30,7 +31,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
   const int col = static_cast<int>(i - token * vectors) * 8;
   const long long pairs = static_cast<long long>(p.tokens) * p.top_k;
   float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
+#pragma unroll 8
   for (int j = 0; j < p.top_k; ++j) {
     const long long row = __ldg(p.positions + token * p.top_k + j);
     const float w = __ldg(p.weights + token * p.top_k + j);
@@ -47,8 +48,8 @@ template <typename T>
 cudaError_t launch_combine(const CombineParams& p, cudaStream_t stream) {
   const long long threads = static_cast<long long>(p.tokens) * (p.dim >> 3);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((threads + 255) / 256));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(static_cast<unsigned>((threads + kCombineThreads - 1) / kCombineThreads));
+  cfg.blockDim = dim3(kCombineThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -498,14 +498,22 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         // h = act(up) * up_v of this warp's features; the block's maximum with the row's other warps
         const int col = t.n0 + column0;
         uint32_t amax = 0;
+        if (any_live) {
+          if (t.n0 + kTileN > p.n) {   // features that do not exist: act(0) is 0
 #pragma unroll
-        for (int j = 0; j < kRun / 2; ++j) {
-          const float2 g = unpack2(acc[j]), w = unpack2(acc[kRun / 2 + j]);
-          float h0 = activate(g.x, p.act), h1 = activate(g.y, p.act);
-          if (second) { h0 *= w.x; h1 *= w.y; }
-          if (col + 2 * j >= p.n) h0 = h1 = 0.0f;   // (n is even)
-          amax = max(amax, max(abs_bits(h0), abs_bits(h1)));
-          acc[j] = pack2(h0, h1);
+            for (int j = 0; j < kRun / 2; ++j)
+              if (col + 2 * j >= p.n) acc[j] = acc[kRun / 2 + j] = 0;   // (n is even)
+          }
+          with_activation(p.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < kRun / 2; ++j) {
+              const float2 g = unpack2(acc[j]), w = unpack2(acc[kRun / 2 + j]);
+              float h0 = activate<decltype(act)::value>(g.x), h1 = activate<decltype(act)::value>(g.y);
+              if (second) { h0 *= w.x; h1 *= w.y; }
+              amax = max(amax, max(abs_bits(h0), abs_bits(h1)));
+              acc[j] = pack2(h0, h1);
+            }
+          });
         }
         sh.amax[parity][column_warp][r] = amax;
         __syncwarp();
@@ -893,18 +901,23 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
       const int row0 = t.row0 + half * kPart + from, live = min(count, t.row_end - row0);   // (may be none)
       if constexpr (kGated) {
         uint32_t* amax = sh.amax[parity][half * 4 + quarter];
+        if (feature >= p.n) {   // act(0) is 0
 #pragma unroll
-        for (int j = 0; j < kPart; ++j) {
-          if (j < live) {   // (the same for the whole warp)
-            const float2 g = unpack2(acc[0][j / 2]), u = unpack2(acc[1][j / 2]);
-            float h = activate(j & 1 ? g.y : g.x, p.act);
-            if (second) h *= j & 1 ? u.y : u.x;
-            if (feature >= p.n) h = 0.0f;
-            acc[0][j / 2] = j & 1 ? pack2(g.x, h) : pack2(h, g.y);
-            const uint32_t m = __reduce_max_sync(0xffffffffu, abs_bits(h));
-            if (lane == 0) amax[j] = m;
-          }
+          for (int j = 0; j < kPart / 2; ++j) acc[0][j] = acc[1][j] = 0;
         }
+        with_activation(p.act, [&](auto act) {
+#pragma unroll
+          for (int j = 0; j < kPart; ++j) {
+            if (j < live) {   // (the same for the whole warp)
+              const float2 g = unpack2(acc[0][j / 2]), u = unpack2(acc[1][j / 2]);
+              float h = activate<decltype(act)::value>(j & 1 ? g.y : g.x);
+              if (second) h *= j & 1 ? u.y : u.x;
+              acc[0][j / 2] = j & 1 ? pack2(g.x, h) : pack2(h, g.y);
+              const uint32_t m = __reduce_max_sync(0xffffffffu, abs_bits(h));
+              if (lane == 0) amax[j] = m;
+            }
+          }
+        });
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.amax_full[half]);
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.amax_full[half], parity, wc));
