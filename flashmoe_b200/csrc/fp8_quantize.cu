@@ -8,6 +8,9 @@ namespace {
 
 constexpr int kMaxDevices = 64;
 
+// From this many blocks on (the GPU full of threads twice over) a thread takes two.
+constexpr long long kTwiceFrom = 2 * 148 * 64 * 4;
+
 struct QuantizeParams {
   const void* x;
   unsigned char* q;
@@ -71,33 +74,43 @@ struct Raw16 {
   }
 };
 
-// Eight threads a block of 128, sixteen values each.
-template <typename T>
+// Eight threads a block of 128, sixteen values each; kTwice: two blocks a thread, both loaded before either is used.
+template <typename T, bool kTwice>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams p) {
   launch_dependents();   // (of the expert layer: its next kernel)
-  const uint32_t block = blockIdx.x * (256 / 8) + (threadIdx.x >> 3);   // (the host sees to it that it fits)
+  constexpr int kEach = kTwice ? 2 : 1, kBlocks = 32 * kEach;   // blocks of a thread, of a CTA
   const int sub = threadIdx.x & 7;
-  const uint32_t row32 = block / static_cast<uint32_t>(p.col_blocks);
-  const long long row = row32;
-  const int cb = static_cast<int>(block - row32 * p.col_blocks), col = cb * kBlock + sub * 16;
-  const bool in = row < p.rows && col < p.cols;   // (cols is a multiple of 16)
-  Raw16<T> raw;
-  raw.zero();
-  if (in) raw.load(static_cast<const T*>(p.x) + row * p.cols + col);
-  uint32_t m = raw.amax_bits();
+  Raw16<T> raw[kEach];
+  uint32_t row[kEach];
+  int cb[kEach], col[kEach];
+  bool in[kEach];
 #pragma unroll
-  for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-  const float amax = Raw16<T>::amax_value(m);
-  const uint4 codes = raw.codes(Quantizer(amax));
-  if (row >= p.rows) return;
-  for (int j = 0; j < p.copies; ++j) {
-    long long to = row;
-    if (p.positions != nullptr) {
-      to = __ldg(p.positions + row * p.copies + j);
-      if (to < 0 || to >= static_cast<long long>(p.rows) * p.copies) continue;
+  for (int i = 0; i < kEach; ++i) {
+    const uint32_t block = blockIdx.x * kBlocks + 32 * i + (threadIdx.x >> 3);   // (the host sees to it that it fits)
+    row[i] = block / static_cast<uint32_t>(p.col_blocks);
+    cb[i] = static_cast<int>(block - row[i] * p.col_blocks);
+    col[i] = cb[i] * kBlock + sub * 16;
+    in[i] = row[i] < static_cast<uint32_t>(p.rows) && col[i] < p.cols;   // (cols is a multiple of 16)
+    raw[i].zero();
+    if (in[i]) raw[i].load(static_cast<const T*>(p.x) + static_cast<size_t>(row[i]) * p.cols + col[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    uint32_t m = raw[i].amax_bits();
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float amax = Raw16<T>::amax_value(m);
+    const uint4 codes = raw[i].codes(Quantizer(amax));
+    if (row[i] >= static_cast<uint32_t>(p.rows)) continue;
+    for (int j = 0; j < p.copies; ++j) {
+      long long to = row[i];
+      if (p.positions != nullptr) {
+        to = __ldg(p.positions + static_cast<size_t>(row[i]) * p.copies + j);
+        if (to < 0 || to >= static_cast<long long>(p.rows) * p.copies) continue;
+      }
+      if (in[i]) *reinterpret_cast<uint4*>(p.q + to * p.cols + col[i]) = codes;
+      if (sub == 0) p.scale[to * p.col_blocks + cb[i]] = block_scale(amax);
     }
-    if (in) *reinterpret_cast<uint4*>(p.q + to * p.cols + col) = codes;
-    if (sub == 0) p.scale[to * p.col_blocks + cb] = block_scale(amax);
   }
 }
 
@@ -137,8 +150,9 @@ __global__ void __launch_bounds__(256) quantize_weights_kernel(const QuantizePar
 template <typename T>
 cudaError_t launch(const QuantizeParams& p, int block_rows, int matrices, cudaStream_t stream) {
   if (block_rows == 1) {
-    const long long threads = static_cast<long long>(p.rows) * p.col_blocks * 8;
-    quantize_rows_kernel<T><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, stream>>>(p);
+    const long long blocks = static_cast<long long>(p.rows) * p.col_blocks;
+    if (blocks >= kTwiceFrom) quantize_rows_kernel<T, true><<<static_cast<unsigned>((blocks + 63) / 64), 256, 0, stream>>>(p);
+    else quantize_rows_kernel<T, false><<<static_cast<unsigned>((blocks + 31) / 32), 256, 0, stream>>>(p);
   } else {
     quantize_weights_kernel<T><<<dim3(static_cast<unsigned>(p.row_blocks * p.col_blocks), matrices), 256, 0, stream>>>(p);
   }

@@ -50,6 +50,21 @@ __device__ __forceinline__ float logit_at(const SelectParams& p, size_t i) {
   return sane(x);
 }
 
+// A lane's logits of a row, lane + 32 i, all on their way together (the type is chosen around the loop, not in it: a
+// branch around each load made them wait for one another, 4000 cycles for eight).  -infinity behind the last.
+template <int V>
+__device__ __forceinline__ void load_row(const SelectParams& p, size_t row, int lane, float (&v)[V]) {
+  auto load = [&](const auto* from) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = lane + 32 * i < p.E ? fp8::to_float(__ldg(from + row + lane + 32 * i)) : -INFINITY;
+  };
+  if (p.dtype == FMOE_DT_FP32) load(static_cast<const float*>(p.logits));
+  else if (p.dtype == FMOE_DT_BF16) load(static_cast<const __nv_bfloat16*>(p.logits));
+  else load(static_cast<const __half*>(p.logits));
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = sane(v[i]);
+}
+
 // An unsigned number that orders like the value (+0 and -0 alike); 0 is left for "nothing".
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
@@ -63,14 +78,20 @@ template <typename F>
 __device__ __forceinline__ F exp_of(F x) {
   if constexpr (sizeof(F) == 8) return exp(x); else return expf(x);
 }
-// exp(l - largest) or sigmoid(l); 0 for a masked logit
+// exp(l - largest) or sigmoid(l); 0 for a masked logit.  In fp32 sigmoid is taken from exp(-|l|), which cannot
+// overflow, without a branch on the sign.
 template <typename F>
 __device__ __forceinline__ F raw_score(F l, F largest, int score) {
-  if (l == -INFINITY) return 0;
-  if (score == FMOE_SCORE_SOFTMAX) return exp_of<F>(l - largest);
-  if (sizeof(F) == 8 || l >= 0) return F(1) / (F(1) + exp_of<F>(-l));
-  const F e = exp_of<F>(l);   // (exp(-l) would overflow fp32 from -89 on)
-  return e / (F(1) + e);
+  F s;
+  if (score == FMOE_SCORE_SOFTMAX) {
+    s = exp_of<F>(l - largest);
+  } else if constexpr (sizeof(F) == 8) {
+    s = 1.0 / (1.0 + exp(-l));
+  } else {
+    const float e = expf(-fabsf(l));
+    s = __fdividef(l >= 0.0f ? 1.0f : e, 1.0f + e);
+  }
+  return l == -INFINITY ? F(0) : s;
 }
 
 template <typename F>
@@ -89,8 +110,9 @@ __device__ __forceinline__ F warp_max(F v) {
   return v;
 }
 
-// A group's score from its experts' values in shared memory: teams of lanes, one a group, walk the
-// values and keep the two largest.  Lane g < groups leaves with group g's score.
+// A group's score from its experts' values in shared memory (each group's run one place longer than it has to be, so
+// that the groups fall on different banks): teams of lanes, one a group, walk the values and keep the two
+// largest.  Lane g < groups leaves with group g's score.
 template <typename F>
 __device__ __forceinline__ F group_score(const F* row, int E, int groups, bool largest_only, int lane) {
   int team = 32;
@@ -99,7 +121,7 @@ __device__ __forceinline__ F group_score(const F* row, int E, int groups, bool l
   F a = -INFINITY, b = -INFINITY;   // the largest two
   if (g < groups) {
     for (int j = sub; j < size; j += team) {
-      const F v = row[g * size + j];
+      const F v = row[g * (size + 1) + j];
       if (v > a) { b = a; a = v; } else if (v > b) { b = v; }
     }
   }
@@ -125,17 +147,25 @@ __device__ __forceinline__ uint32_t kept_groups(F mine, int groups, int top_grou
   return __ballot_sync(kAll, stays);
 }
 
+// The group of expert e: (e + 1/2) / size lies at least 1/2048 from a whole number, fp32 is exact to far less.
+__device__ __forceinline__ int group_of(int e, float groups_per_expert) {
+  return static_cast<int>((static_cast<float>(e) + 0.5f) * groups_per_expert);
+}
 // Bits i of the experts lane + 32 i that exist and whose group stays.
 template <int V>
 __device__ __forceinline__ uint32_t alive_bits(int E, int groups, uint32_t kept, int lane) {
   uint32_t alive = 0;
+  if (groups == 1) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (lane + 32 * i < E) alive |= 1u << i;
+    return alive;
+  }
   const float per = static_cast<float>(groups) / static_cast<float>(E);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int e = lane + 32 * i;
-    // (e + 1/2) / size lies at least 1/2048 from a whole number, fp32 is exact to far less
-    const int g = static_cast<int>((static_cast<float>(e) + 0.5f) * per);
-    if (e < E && (groups == 1 || (kept >> g & 1))) alive |= 1u << i;
+    if (e < E && (kept >> group_of(e, per) & 1)) alive |= 1u << i;
   }
   return alive;
 }
@@ -169,10 +199,11 @@ __device__ __noinline__ int choose_exactly(const SelectParams& p, size_t row, in
   }
   uint32_t kept = kAll;
   if (p.groups > 1) {
+    const float per = static_cast<float>(p.groups) / static_cast<float>(p.E);
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (lane + 32 * i < p.E) shared_row[lane + 32 * i] = c[i];
+      if (lane + 32 * i < p.E) shared_row[lane + 32 * i + group_of(lane + 32 * i, per)] = c[i];
     __syncwarp();
     double worst, best;
     kept = kept_groups<double>(group_score<double>(shared_row, p.E, p.groups, p.group_max, lane), p.groups, p.top_groups,
@@ -202,17 +233,17 @@ __device__ __noinline__ int choose_exactly(const SelectParams& p, size_t row, in
   return mine;
 }
 
-// One token by one warp: ids and weights.  shared_row: E doubles, used with groups only.
+// One token by one warp: ids and weights.  shared_row: row_doubles(E, groups) doubles, used with groups only.
 template <int V>
 __device__ __forceinline__ void select_token(const SelectParams& p, int token, int lane, double* shared_row) {
   const size_t row = static_cast<size_t>(token) * p.E;
   const bool softmax = p.score == FMOE_SCORE_SOFTMAX, by_score = p.bias != nullptr || p.groups > 1;
-  float v[V];
+  float v[V], bias[V];
+  if (p.bias != nullptr) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = lane + 32 * i;
-    v[i] = e < p.E ? logit_at(p, row + e) : -INFINITY;
+    for (int i = 0; i < V; ++i) bias[i] = lane + 32 * i < p.E ? __ldg(p.bias + lane + 32 * i) : 0.0f;
   }
+  load_row<V>(p, row, lane, v);
   float top = -INFINITY;
   if (softmax && (by_score || !p.renormalize)) {
 #pragma unroll
@@ -239,17 +270,17 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
   if (by_score) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = lane + 32 * i;
-      if (softmax && sum > 0.0f) c[i] = c[i] / sum;
+      if (softmax && sum > 0.0f) c[i] = __fdividef(c[i], sum);
       if (v[i] == -INFINITY) c[i] = -INFINITY;
-      if (p.bias != nullptr && e < p.E) c[i] += sane(__ldg(p.bias + e));
+      if (p.bias != nullptr) c[i] += sane(bias[i]);
     }
     if (p.groups > 1) {
       float* shared = reinterpret_cast<float*>(shared_row);
+      const float per = static_cast<float>(p.groups) / static_cast<float>(p.E);
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (lane + 32 * i < p.E) shared[lane + 32 * i] = c[i];
+        if (lane + 32 * i < p.E) shared[lane + 32 * i + group_of(lane + 32 * i, per)] = c[i];
       __syncwarp();
       float worst, best;
       kept = kept_groups<float>(group_score<float>(shared, p.E, p.groups, p.group_max, lane), p.groups, p.top_groups, lane,
@@ -272,27 +303,41 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
     keys[i] = alive >> i & 1 ? order_key(c[i]) : 0;
     at[i] = lane + 32 * i;
   }
-  // odd-even transposition: neighbours only, so equal keys keep their order
+  constexpr bool kSorted = V <= 8;   // sorting 16 takes 120 exchanges, more than looking for the best nine times
+  if constexpr (kSorted) {
+    // odd-even transposition: neighbours only, so equal keys keep their order
 #pragma unroll
-  for (int pass = 0; pass < V; ++pass)
+    for (int pass = 0; pass < V; ++pass)
 #pragma unroll
-    for (int i = pass & 1; i + 1 < V; i += 2) {
-      const bool swap = keys[i + 1] > keys[i];
-      const uint32_t hi = swap ? keys[i + 1] : keys[i], lo = swap ? keys[i] : keys[i + 1];
-      const int first = swap ? at[i + 1] : at[i], then = swap ? at[i] : at[i + 1];
-      keys[i] = hi; keys[i + 1] = lo;
-      at[i] = first; at[i + 1] = then;
-    }
+      for (int i = pass & 1; i + 1 < V; i += 2) {
+        const bool swap = keys[i + 1] > keys[i];
+        const uint32_t hi = swap ? keys[i + 1] : keys[i], lo = swap ? keys[i] : keys[i + 1];
+        const int first = swap ? at[i + 1] : at[i], then = swap ? at[i] : at[i + 1];
+        keys[i] = hi; keys[i + 1] = lo;
+        at[i] = first; at[i + 1] = then;
+      }
+  }
+  uint32_t head = keys[0];
+  int head_at = at[0];
+  auto find_head = [&] {
+    head = keys[0];
+    head_at = lane;
+#pragma unroll
+    for (int i = 1; i < V; ++i)
+      if (keys[i] > head) { head = keys[i]; head_at = lane + 32 * i; }
+  };
+  if constexpr (!kSorted) find_head();
   // Lane r gets the r-th candidate.  By score there is at least one more than k, and more as long as the last two
   // are too close to tell apart (up to the warp's 32).
   int mine = 0, found = 0;
+  uint32_t mine_key = 0;
   float last = 0.0f;
   bool close = false;
   for (;; ++found) {
     if (by_logit && found == p.k) break;
-    const uint32_t key = __reduce_max_sync(kAll, keys[0]);
+    const uint32_t key = __reduce_max_sync(kAll, head);
     if (key == 0) break;                         // every expert is taken
-    const int e = __reduce_min_sync(kAll, keys[0] == key ? at[0] : 0x7fffffff);
+    const int e = __reduce_min_sync(kAll, head == key ? head_at : 0x7fffffff);
     if (!by_logit) {
       const float now = key_value(key);
       const bool near = found > 0 && last - now <= 2.0f * error + 0x1p-23f * fmaxf(fabsf(last), fabsf(now));
@@ -301,14 +346,26 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
       last = now;
       if (found == 32) { unsure = true; break; }
     }
-    if (lane == found) mine = e;
-    const bool took = lane == (e & 31);
-#pragma unroll
-    for (int i = 0; i + 1 < V; ++i) {
-      keys[i] = took ? keys[i + 1] : keys[i];
-      at[i] = took ? at[i + 1] : at[i];
+    if (lane == found) {
+      mine = e;
+      mine_key = key;
     }
-    keys[V - 1] = took ? 0 : keys[V - 1];
+    const bool took = lane == (e & 31);
+    if constexpr (kSorted) {
+#pragma unroll
+      for (int i = 0; i + 1 < V; ++i) {
+        keys[i] = took ? keys[i + 1] : keys[i];
+        at[i] = took ? at[i + 1] : at[i];
+      }
+      keys[V - 1] = took ? 0 : keys[V - 1];
+      head = keys[0];
+      head_at = at[0];
+    } else if (took) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i == e >> 5) keys[i] = 0;
+      find_head();
+    }
   }
   if (unsure) {                                  // (the same for the whole warp, as everything that follows)
     mine = choose_exactly<V>(p, row, lane, shared_row);
@@ -345,7 +402,8 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
     }
     mine = sorted;
   }
-  const float l = lane < p.k ? logit_at(p, row + mine) : -INFINITY;
+  float l = -INFINITY;
+  if (lane < p.k) l = by_logit && !unsure ? key_value(mine_key) : logit_at(p, row + mine);
   // (shares among the chosen do not depend on the largest of all, which may be far above theirs)
   float s = raw_score<float>(l, p.renormalize ? (by_logit ? __shfl_sync(kAll, l, 0) : warp_max<float>(l)) : top, p.score);
   if (softmax && !p.renormalize && sum > 0.0f) s = s / sum;
@@ -359,18 +417,20 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
   }
 }
 
+__host__ __device__ __forceinline__ size_t row_doubles(int E, int groups) { return groups > 1 ? E + groups : 0; }
+
 template <int V>
 __global__ void __launch_bounds__(256) select_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ __align__(16) unsigned char s_raw[];
   fp8::launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.x * 8 + warp;
-  if (token < p.S) select_token<V>(p, token, lane, reinterpret_cast<double*>(s_raw) + static_cast<size_t>(warp) * p.E);
+  if (token < p.S) select_token<V>(p, token, lane, reinterpret_cast<double*>(s_raw) + warp * row_doubles(p.E, p.groups));
 }
 
 // ---- ordering ---------------------------------------------------------------------------------------
 
-constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32, kOrderCtas = 8;
+constexpr int kOrderThreads = 1024, kOrderWarps = kOrderThreads / 32;
 constexpr int kAhead = 8;   // pairs a lane loads before it uses the first
 
 // What is known of pair i: its expert e, its slot there, and the first row of the expert.
@@ -437,13 +497,17 @@ __device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bo
   __syncthreads();
   const int e = threadIdx.x;                      // (at most kOrderThreads experts)
   if (e < E) {
-    int c[kOrderWarps], sum = 0;
+    int sum = 0;
 #pragma unroll
-    for (int w = 0; w < kOrderWarps; ++w) c[w] = hist[w * E + e];
+    for (int w0 = 0; w0 < kOrderWarps; w0 += 16) {
+      int c[16];
 #pragma unroll
-    for (int w = 0; w < kOrderWarps; ++w) {
-      hist[w * E + e] = sum;
-      sum += c[w];
+      for (int w = 0; w < 16; ++w) c[w] = hist[(w0 + w) * E + e];
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        hist[(w0 + w) * E + e] = sum;
+        sum += c[w];
+      }
     }
     total[e] = sum;
   }
@@ -512,10 +576,10 @@ __device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bo
   }
 }
 
+template <int kCtas>
 __global__ void __launch_bounds__(kOrderThreads) order_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ __align__(16) unsigned char s_raw[];
-  if (gridDim.x == 1) order_pairs<1>(p, reinterpret_cast<int*>(s_raw), p.S > 0);
-  else order_pairs<kOrderCtas>(p, reinterpret_cast<int*>(s_raw), p.S > 0);
+  order_pairs<kCtas>(p, reinterpret_cast<int*>(s_raw), p.S > 0);
 }
 
 // Few tokens: one CTA chooses and orders.
@@ -524,7 +588,7 @@ __global__ void __launch_bounds__(kOrderThreads) select_few_kernel(const __grid_
   extern __shared__ __align__(16) unsigned char s_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int token = warp; token < p.S; token += kOrderWarps)
-    select_token<V>(p, token, lane, reinterpret_cast<double*>(s_raw) + static_cast<size_t>(warp) * p.E);
+    select_token<V>(p, token, lane, reinterpret_cast<double*>(s_raw) + warp * row_doubles(p.E, p.groups));
   __syncthreads();
   order_pairs<1>(p, reinterpret_cast<int*>(s_raw), false);
 }
@@ -565,7 +629,7 @@ constexpr int kFewTokens = 64;
 
 template <int V>
 cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
-  const size_t group_row = p.groups > 1 ? static_cast<size_t>(p.E) * sizeof(double) : 0;
+  const size_t group_row = row_doubles(p.E, p.groups) * sizeof(double);
   const size_t order = static_cast<size_t>(kOrderWarps + 1) * p.E * sizeof(int);
   if constexpr (V <= 8) {   // (the registers of 32 warps)
     if (p.S <= kFewTokens) {
@@ -577,8 +641,12 @@ cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
     const cudaError_t e = launch(select_kernel<V>, p, (p.S + 7) / 8, 256, 8 * group_row, 1, false, stream);
     if (e != cudaSuccess) return e;
   }
-  const int ctas = static_cast<long long>(p.S) * p.k <= kOrderThreads ? 1 : kOrderCtas;
-  return launch(order_kernel, p, ctas, kOrderThreads, order, ctas, p.S > 0, stream);
+  // (both kernels, 65536 pairs of 128 experts: 18.5 us by 8 CTAs, 16.4 by 16; 16384 pairs of 256 experts: 15.1 and 14.4)
+  const long long pairs = static_cast<long long>(p.S) * p.k;
+  if (pairs <= kOrderThreads) return launch(order_kernel<1>, p, 1, kOrderThreads, order, 1, p.S > 0, stream);
+  const cudaError_t e = cudaFuncSetAttribute(order_kernel<16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  return launch(order_kernel<16>, p, 16, kOrderThreads, order, 16, p.S > 0, stream);
 }
 
 int check(const fmoe_select_args* a) {
