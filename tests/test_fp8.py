@@ -244,6 +244,47 @@ def test_product_by_expert(counts, n, k, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("counts,n,k", [([20], 512, 4096), ([3], 300, 8192), ([300], 777, 2064), ([520], 1032, 4096), ([900], 4112, 528),
+                                        ([2304], 4864, 4112), ([2500], 9500, 2064), ([70] * 20, 1024, 1040), ([90] * 24, 1024, 1040),
+                                        ([2000, 3000], 4864, 2064), ([0, 3000, 3500], 8192, 4112)],
+                         ids=["16 rows, split", "16 rows, split more", "32 rows, split", "64 rows", "128 rows", "pairs", "pairs, odd rows",
+                              "64 rows, experts", "128 rows, experts", "128 rows, few experts", "pairs, few experts"])
+def test_every_tile_form(counts, n, k, dtype):
+    """Sizes that take each of the kernels (what takes which is the library's choice: the results are what is held here)."""
+    spans = spans_of(counts)
+    m = spans[-1]
+    a, sa = rows8(m, k, m)
+    w, sw = weights8(len(counts), n, k, n)
+    off = torch.tensor(spans, dtype=torch.int32, device="cuda") if len(counts) > 1 else None
+    want, mag = product64(a, sa, w, sw, spans)
+    close(run_matmul(a, sa, w, sw, dtype, off), want, sum_tol(k) * mag, dtype)
+    assert fp8.last_status(0, stream()).code == 0
+
+
+@gpu
+def test_places_beyond_32_bits():
+    """More than 2^31 values in and out: the last rows land where they belong."""
+    rows, cols = 270_000, 8192
+    x = torch.zeros(1, rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[0, -3:] = normal((3, cols), 1, dtype=torch.bfloat16)
+    q = torch.zeros(1, rows, cols, dtype=E4M3, device="cuda")
+    s = torch.full((1, rows, blocks(cols)), -7.0, device="cuda")
+    fp8.quantize(fp8.QuantizeArgs(x.data_ptr(), q.data_ptr(), s.data_ptr(), stream(), rows=rows, cols=cols))
+    torch.cuda.synchronize()
+    want_q, want_s = plain_quantize(x[:, -3:], 1)
+    assert same(q[0, -3:], want_q[0]) and torch.equal(s[0, -3:], want_s[0]) and not s[0, :-3].any()
+    del x, q, s
+    m, n, k = 66_000, 33_000, 16
+    a, sa = rows8(m, k, 2)
+    w, sw = weights8(1, n, k, 3)
+    out = run_matmul(a, sa, w, sw, torch.bfloat16)
+    for r in (slice(0, 2), slice(m // 2, m // 2 + 2), slice(m - 2, m)):
+        want, mag = product64(a[r], sa[r], w, sw, [0, 2])
+        close(out[r], want, sum_tol(k) * mag, torch.bfloat16)
+
+
+@gpu
 def test_no_rows_and_offsets_outside_the_rows():
     k, n = 256, 128
     a, sa = rows8(20, k, 1)
@@ -341,7 +382,8 @@ def check_gated(q, s, m, g, tg, u, tu, k, act):
 @pytest.mark.parametrize("act", list(ActivationType), ids=lambda a: a.name)
 @pytest.mark.parametrize("gated", [True, False])
 @pytest.mark.parametrize("counts,n,k", [([1], 16, 16), ([5], 144, 256), ([64], 384, 272), ([200], 272, 1024), ([2, 0, 40, 1], 256, 384),
-                                        ([130, 7, 0], 400, 512), ([1] * 40, 128, 144)], ids=str)
+                                        ([130, 7, 0], 400, 512), ([1] * 40, 128, 144), ([5], 256, 4096), ([100], 1040, 2064),
+                                        ([300], 2064, 2064), ([40] * 6, 2048, 1040)], ids=str)
 def test_gated_product(counts, n, k, gated, act):
     spans = spans_of(counts)
     m, E = spans[-1], len(counts)
@@ -358,6 +400,20 @@ def test_gated_product(counts, n, k, gated, act):
     cut = lambda t: None if t is None else t[:m]
     check_gated(q, s, m, cut(g), cut(tg), cut(u), cut(tu), k, act)
     assert bool((q[m:].float() == 1.0).all()) and bool((s[m:] == -7.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("gated", [True, False])
+def test_gated_product_by_pairs(gated):
+    counts, n, k = [2000, 3000], 4864, 2064
+    spans, act = spans_of(counts), ActivationType.SILU
+    a, sa = rows8(5000, k, 1)
+    up, sup = weights8(2, n, k, 2)
+    v, sv = weights8(2, n, k, 3) if gated else (None, None)
+    q, s = run_gated(a, sa, up, sup, v, sv, act, torch.tensor(spans, dtype=torch.int32, device="cuda"))
+    g, tg = product64(a, sa, up, sup, spans)
+    u, tu = product64(a, sa, v, sv, spans) if gated else (None, None)
+    check_gated(q, s, 5000, g, tg, u, tu, k, act)
 
 
 # ---- the layer ---------------------------------------------------------------------------------------------
@@ -464,6 +520,38 @@ def test_two_layers_at_once_on_two_streams():
 
 
 @gpu
+def test_two_graphs_and_eager_calls_of_one_layer():
+    """Two captured steps and eager ones, ordered by one stream, share the layer's workspace and outputs."""
+    side = torch.cuda.Stream()
+    layer = Layer(24, 256, 272, 8, 2, stream_ptr=side.cuda_stream)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            layer.step()
+        graphs.append(g)
+    for seed, run in enumerate([graphs[0].replay, layer.step, graphs[1].replay, graphs[0].replay, layer.step]):
+        layer.x.copy_(normal((24, 256), 50 + seed, dtype=torch.bfloat16))
+        layer.logits.copy_(normal((24, 8), 80 + seed))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.synchronize()
+        layer.check()
+
+
+@gpu
+def test_large_layer_on_every_form():
+    """4096 tokens on 4 experts (pairs) and 64 experts (128 rows)."""
+    for E, k in ((4, 2), (64, 2)):
+        layer = Layer(4096, 512, 640, E, k, seed=E)
+        layer.step()
+        torch.cuda.synchronize()
+        layer.check()
+
+
+@gpu
 def test_no_tokens():
     layer = Layer(0, 64, 64, 8, 2)
     layer.step()
@@ -532,6 +620,11 @@ def test_experts_refusals(kw, code, needle):
     a.update(kw)
     pos = [a.pop(n) for n in names] + [a.pop("workspace_bytes")]
     refused(fp8.experts, fp8.ExpertsArgs(*pos, 0, **a), code, needle)
+
+
+def test_last_status_refusals():
+    assert N.lib().fmoe_fp8_last_status(0, None, None) == 1
+    assert N.lib().fmoe_fp8_last_status(64, None, C.byref(N.Status())) == 1
 
 
 def test_workspace_bytes():
