@@ -209,6 +209,7 @@ __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontr
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---- host side -----------------------------------------------------------------------------------
+constexpr int kMaxDevices = 64;
 // Makes `device` current for the scope and puts the caller's device back.
 struct OnDevice {
   int prev = -1;
@@ -226,10 +227,11 @@ struct OnDevice {
   OnDevice& operator=(const OnDevice&) = delete;
 };
 inline bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
-// The products, launched under the tail of the stream's last kernel where `dependent`: that kernel must have been
-// launched after everything but A was complete, and write A.
-int matmul(const fmoe_fp8_matmul_args* a, bool dependent, cudaStream_t stream);
-int gated_matmul(const fmoe_fp8_gated_args* a, bool dependent, cudaStream_t stream);
+// The products.  kDependent: launched under the tail of the stream's last kernel, which writes A and was itself launched
+// after everything else was complete; kCheckOnly: the arguments are looked at, nothing is launched.
+enum class Launch { kPlain, kDependent, kCheckOnly };
+int matmul(const fmoe_fp8_matmul_args* a, Launch how, cudaStream_t stream);
+int gated_matmul(const fmoe_fp8_gated_args* a, Launch how, cudaStream_t stream);
 inline int element_bytes(int data_type) { return data_type == FMOE_DT_FP32 ? 4 : 2; }
 
 }  // namespace fmoe::fp8

@@ -9,7 +9,6 @@
 namespace fmoe::fp8 {
 namespace {
 
-constexpr int kMaxDevices = 64;
 constexpr int kCombineThreads = 128;
 
 struct CombineParams {
@@ -89,7 +88,7 @@ int check_shape(const fmoe_fp8_experts_args* a) {
     return set_error(FMOE_ERR_INVALID_ARG, "top_k must not exceed num_experts (or 32)");
   if (a->data_type != FMOE_DT_BF16 && a->data_type != FMOE_DT_FP16)
     return set_error(FMOE_ERR_UNSUPPORTED, "the 8-bit expert layer handles BF16 and FP16 tokens");
-  if (static_cast<long long>(a->num_tokens) * a->top_k > 0x7fffff00ll)
+  if (static_cast<long long>(a->num_tokens) * a->top_k > 0x7fff0000ll)
     return set_error(FMOE_ERR_UNSUPPORTED, "num_tokens * top_k must fit 32 bits");
   return FMOE_OK;
 }
@@ -137,15 +136,18 @@ int fmoe_fp8_experts(const fmoe_fp8_experts_args* a, void* stream) {
                                   a->token_dim, a->num_experts, a->act_type, a->device_id};
   const fmoe_fp8_matmul_args down{ws + pl.hq, reinterpret_cast<float*>(ws + pl.hs), a->down, a->down_scale, ws + pl.y, a->offsets,
                                   pairs, a->token_dim, a->ffn_size, a->num_experts, a->data_type, a->device_id};
-  rc = fmoe_fp8_quantize(&quantize, stream);
-  if (rc == FMOE_OK) rc = gated_matmul(&gated, true, static_cast<cudaStream_t>(stream));
-  if (rc == FMOE_OK) rc = matmul(&down, true, static_cast<cudaStream_t>(stream));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  rc = gated_matmul(&gated, Launch::kCheckOnly, st);   // what any of the steps refuses is refused before the first
+  if (rc == FMOE_OK) rc = matmul(&down, Launch::kCheckOnly, st);
+  if (rc == FMOE_OK) rc = fmoe_fp8_quantize(&quantize, stream);
+  if (rc == FMOE_OK) rc = gated_matmul(&gated, Launch::kDependent, st);
+  if (rc == FMOE_OK) rc = matmul(&down, Launch::kDependent, st);
   if (rc != FMOE_OK) return rc;
   OnDevice on(a->device_id);
   if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));
   const CombineParams c{ws + pl.y, a->positions, a->weights, a->out, a->num_tokens, a->token_dim, a->top_k};
-  const cudaError_t e = a->data_type == FMOE_DT_BF16 ? launch_combine<__nv_bfloat16>(c, static_cast<cudaStream_t>(stream))
-                                                     : launch_combine<__half>(c, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = a->data_type == FMOE_DT_BF16 ? launch_combine<__nv_bfloat16>(c, st)
+                                                     : launch_combine<__half>(c, st);
   if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("combine launch: ") + cudaGetErrorString(e));
   return FMOE_OK;
 }

@@ -91,7 +91,9 @@ __device__ __forceinline__ bool find_tile(const TileTable& t, const ProductParam
   return true;
 }
 
-// Called by every thread; the tile counts are summed by warp 0.
+// Called by every thread; the tile counts are summed by warp 0.  With offsets that make sense the sums fit (the host
+// checks); with others they stop at a number that a stride of the grid does not overflow.
+constexpr long long kMostTiles = 0x7fff0000;
 __device__ void fill_table(TileTable& t, const ProductParams& p, int tile_m) {
   for (int e = threadIdx.x; e < p.experts; e += blockDim.x) {
     int begin, end;
@@ -100,20 +102,20 @@ __device__ void fill_table(TileTable& t, const ProductParams& p, int tile_m) {
   }
   __syncthreads();
   if (threadIdx.x < 32) {
-    int before = 0;
+    long long before = 0;
     for (int e0 = 0; e0 < p.experts; e0 += 32) {
       const int e = e0 + threadIdx.x;
       const int own = e < p.experts ? t.first[e] : 0;
-      int sum = own;
+      long long sum = own;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, d);
+        const long long v = __shfl_up_sync(0xffffffffu, sum, d);
         if (static_cast<int>(threadIdx.x) >= d) sum += v;
       }
-      if (e < p.experts) t.first[e] = before + sum - own;
+      if (e < p.experts) t.first[e] = static_cast<int>(min(before + sum - own, kMostTiles));
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (threadIdx.x == 0) t.first[p.experts] = before;
+    if (threadIdx.x == 0) t.first[p.experts] = static_cast<int>(min(before, kMostTiles));
   }
   __syncthreads();
 }
@@ -974,7 +976,6 @@ struct DeviceFacts {
   int sms = 0;
   long long spin_limit = 0;
 };
-constexpr int kMaxDevices = 64;
 const DeviceFacts& facts(int device) {
   static DeviceFacts all[kMaxDevices];
   static std::once_flag once[kMaxDevices];
@@ -1119,9 +1120,8 @@ int check_product(const void* a, const float* a_scale, const void* w, const floa
   if (device < 0 || device >= kMaxDevices) return set_error(FMOE_ERR_INVALID_ARG, "device_id out of range");
   if (k % 16 != 0) return set_error(FMOE_ERR_INVALID_ARG, "k must be a multiple of 16");
   if (experts > 1 && offsets == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "several experts need offsets");
-  const long long row_tiles = static_cast<long long>(m) / 16 + experts;
-  if (static_cast<long long>(experts) * n > 0x7fffff00ll || row_tiles * (n / 128 + 1) * experts > 0x7fffffffll ||
-      m > 0x7fffff00)
+  const long long tiles = (static_cast<long long>(m) / 16 + experts) * (n / 128 + 1);
+  if (m > kMostTiles || static_cast<long long>(experts) * n > kMostTiles || tiles > kMostTiles)
     return set_error(FMOE_ERR_UNSUPPORTED, "more rows, features or tiles than 32-bit tile numbers hold");
   if (m > 0 && (a == nullptr || a_scale == nullptr || w == nullptr || w_scale == nullptr))
     return set_error(FMOE_ERR_INVALID_ARG, "both operands and their scales are required");
@@ -1143,7 +1143,7 @@ ProductParams product_params(int m, int n, int k, int experts, const int32_t* of
 
 }  // namespace
 
-int matmul(const fmoe_fp8_matmul_args* a, bool dependent, cudaStream_t st) {
+int matmul(const fmoe_fp8_matmul_args* a, Launch how, cudaStream_t st) {
   if (a == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "arguments are null");
   int rc = check_product(a->a, a->a_scale, a->w, a->w_scale, a->offsets, a->m, a->n, a->k, a->num_experts, a->device_id);
   if (rc != FMOE_OK) return rc;
@@ -1153,6 +1153,7 @@ int matmul(const fmoe_fp8_matmul_args* a, bool dependent, cudaStream_t st) {
   if (a->m == 0) return FMOE_OK;
   if (a->out == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "out is required");
   if (misaligned(a->out, eb)) return set_error(FMOE_ERR_INVALID_ARG, "out must be aligned to its type");
+  if (how == Launch::kCheckOnly) return FMOE_OK;
   OnDevice on(a->device_id);
   if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));
   ProductParams p = product_params(a->m, a->n, a->k, a->num_experts, a->offsets, a->device_id);
@@ -1160,13 +1161,13 @@ int matmul(const fmoe_fp8_matmul_args* a, bool dependent, cudaStream_t st) {
   p.w_scale[0] = a->w_scale;
   p.out = a->out;
   p.wide = !misaligned(a->out, 32) && (static_cast<size_t>(a->n) * eb) % 32 == 0;
-  p.dependent = dependent;
+  p.dependent = how == Launch::kDependent;
   if (a->data_type == FMOE_DT_BF16) return launch_product<__nv_bfloat16>(p, a->a, a->w, a->w, a->device_id, st);
   if (a->data_type == FMOE_DT_FP16) return launch_product<__half>(p, a->a, a->w, a->w, a->device_id, st);
   return launch_product<float>(p, a->a, a->w, a->w, a->device_id, st);
 }
 
-int gated_matmul(const fmoe_fp8_gated_args* a, bool dependent, cudaStream_t st) {
+int gated_matmul(const fmoe_fp8_gated_args* a, Launch how, cudaStream_t st) {
   if (a == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "arguments are null");
   int rc = check_product(a->a, a->a_scale, a->up, a->up_scale, a->offsets, a->m, a->ffn_size, a->k, a->num_experts,
                          a->device_id);
@@ -1180,6 +1181,7 @@ int gated_matmul(const fmoe_fp8_gated_args* a, bool dependent, cudaStream_t st) 
   if (misaligned(a->scale, 4) || misaligned(a->up_v_scale, 4))
     return set_error(FMOE_ERR_INVALID_ARG, "scales must be 4-byte aligned");
   if (a->up_v != nullptr && a->up_v_scale == nullptr) return set_error(FMOE_ERR_INVALID_ARG, "up_v needs its scales");
+  if (how == Launch::kCheckOnly) return FMOE_OK;
   OnDevice on(a->device_id);
   if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));
   ProductParams p = product_params(a->m, a->ffn_size, a->k, a->num_experts, a->offsets, a->device_id);
@@ -1190,7 +1192,7 @@ int gated_matmul(const fmoe_fp8_gated_args* a, bool dependent, cudaStream_t st) 
   p.out_scale = a->scale;
   p.act = a->act_type;
   p.has_v = a->up_v != nullptr;
-  p.dependent = dependent;
+  p.dependent = how == Launch::kDependent;
   return launch_product<Codes>(p, a->a, a->up, a->up_v != nullptr ? a->up_v : a->up, a->device_id, st);
 }
 
@@ -1201,10 +1203,10 @@ using namespace fmoe::fp8;
 
 extern "C" {
 
-int fmoe_fp8_matmul(const fmoe_fp8_matmul_args* a, void* stream) { return matmul(a, false, static_cast<cudaStream_t>(stream)); }
+int fmoe_fp8_matmul(const fmoe_fp8_matmul_args* a, void* stream) { return matmul(a, Launch::kPlain, static_cast<cudaStream_t>(stream)); }
 
 int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* a, void* stream) {
-  return gated_matmul(a, false, static_cast<cudaStream_t>(stream));
+  return gated_matmul(a, Launch::kPlain, static_cast<cudaStream_t>(stream));
 }
 
 int fmoe_fp8_last_status(int32_t device_id, void* stream, fmoe_status* out) {

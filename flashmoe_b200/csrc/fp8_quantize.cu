@@ -6,8 +6,6 @@
 namespace fmoe::fp8 {
 namespace {
 
-constexpr int kMaxDevices = 64;
-
 // From this many blocks on (the GPU full of threads twice over) a thread takes two.
 constexpr long long kTwiceFrom = 2 * 148 * 64 * 4;
 

@@ -19,7 +19,6 @@ namespace fmoe {
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxTopK = 32, kMaxGroups = 32;
-constexpr int kMaxDevices = 64;
 constexpr unsigned kAll = 0xffffffffu;
 
 struct SelectParams {
@@ -666,7 +665,7 @@ int check(const fmoe_select_args* a) {
     return set_error(FMOE_ERR_INVALID_ARG, "unknown group_score");
   if (a->data_type != FMOE_DT_BF16 && a->data_type != FMOE_DT_FP16 && a->data_type != FMOE_DT_FP32)
     return set_error(FMOE_ERR_UNSUPPORTED, "logits are BF16, FP16 or FP32");
-  if (a->device_id < 0 || a->device_id >= kMaxDevices) return set_error(FMOE_ERR_INVALID_ARG, "device_id out of range");
+  if (a->device_id < 0 || a->device_id >= fp8::kMaxDevices) return set_error(FMOE_ERR_INVALID_ARG, "device_id out of range");
   if (static_cast<long long>(a->num_tokens) * a->top_k > 0x7fffffffll)
     return set_error(FMOE_ERR_UNSUPPORTED, "num_tokens * top_k must fit 32 bits");
   if (a->expert_counts == nullptr || (a->num_tokens > 0 && (a->logits == nullptr || a->ids == nullptr || a->weights == nullptr)))

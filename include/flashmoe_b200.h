@@ -286,7 +286,8 @@ typedef struct fmoe_select_args {
   int32_t device_id;       /* of every pointer and of `stream`; the caller's current device is kept */
 } fmoe_select_args;
 /* `moe` (may be null): a context of this shape (S, E, k); its routing table and route records are
- * written too, so that fmoe_forward(moe, ...) on the same stream runs on this choice. */
+ * written too, so that fmoe_forward(moe, ...) on the same stream runs on this choice.  (With top_k 1
+ * fmoe_forward copies an expert's rows unscaled, as ever; fmoe_fp8_experts applies the weight.) */
 int fmoe_router_select(fmoe_ctx* moe, const fmoe_select_args* args, void* stream);
 
 /* --- experts in 8 bits ------------------------------------------------------------------ */

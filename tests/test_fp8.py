@@ -587,7 +587,8 @@ def test_quantize_refusals(kw, code, needle):
     (dict(num_experts=1025, offsets=64), 1, "1024"), (dict(num_experts=2), 1, "offsets"), (dict(data_type=DataType.FP64), 2, "BF16"),
     (dict(a=0), 1, "required"), (dict(out=0), 1, "out"), (dict(w=72), 1, "16-byte"), (dict(out=65), 1, "aligned"),
     (dict(w_scale=2), 1, "4-byte"), (dict(offsets=2), 1, "4-byte"), (dict(device_id=64), 1, "device_id"),
-    (dict(num_experts=1024, n=1 << 22, offsets=64), 2, "32-bit"),
+    (dict(num_experts=1024, n=1 << 22, offsets=64), 2, "32-bit"), (dict(m=0x7fffffff), 2, "32-bit"),
+    (dict(m=1 << 24, n=1 << 24), 2, "32-bit"),
 ])
 def test_matmul_refusals(kw, code, needle):
     a = dict(a=64, a_scale=64, w=64, w_scale=64, out=64, m=4, n=128, k=128)
@@ -611,7 +612,9 @@ def test_gated_refusals(kw, code, needle):
     (dict(num_tokens=-1), 1, "num_tokens"), (dict(token_dim=72), 1, "multiples of 16"), (dict(ffn_size=8), 1, "multiples of 16"),
     (dict(top_k=9), 1, "top_k"), (dict(num_experts=2000), 1, "num_experts"), (dict(data_type=DataType.FP32), 2, "BF16"),
     (dict(workspace_bytes=100), 1, "workspace"), (dict(workspace=0), 1, "workspace"), (dict(workspace=128), 1, "256-byte"),
-    (dict(tokens=0), 1, "required"), (dict(tokens=8), 1, "16-byte"), (dict(positions=2), 1, "4-byte"), (dict(act_type=9), 1, "act_type"),
+    (dict(tokens=0), 1, "required"), (dict(tokens=8), 1, "16-byte"), (dict(positions=2), 1, "4-byte"),
+    (dict(up=8), 1, "16-byte"), (dict(up_v=8, up_v_scale=64), 1, "16-byte"), (dict(up_v=64), 1, "up_v"), (dict(offsets=2), 1, "4-byte"),
+    (dict(down_scale=2), 1, "4-byte"), (dict(num_tokens=1 << 30, workspace_bytes=1 << 60), 2, "32"), (dict(act_type=9), 1, "act_type"),
     (dict(device_id=99), 1, "device_id"),
 ])
 def test_experts_refusals(kw, code, needle):
