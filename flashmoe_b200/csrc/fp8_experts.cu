@@ -4,6 +4,9 @@
 // first weights, before it waits for what that one writes.  The first is an ordinary launch, so whatever the chain
 // reads from outside is complete by then; every CTA of every kernel waits before it ends, so the end of the last one
 // is the end of all.
+//
+// The down product's rows stay in fp32 until they are summed: in 16 bits they would be half the bytes, a few per cent
+// of a large layer's time, and their rounding would add as much error again as the one at the end.
 #include "fp8.cuh"
 
 namespace fmoe::fp8 {
@@ -12,42 +15,42 @@ namespace {
 constexpr int kCombineThreads = 128;
 
 struct CombineParams {
-  const void* y;              // [tokens * top_k, dim], expert order
+  const float* y;             // [tokens * top_k, dim], expert order
   const int32_t* positions;   // [tokens, top_k]
   const float* weights;       // [tokens, top_k]
   void* out;                  // [tokens, dim]
   int tokens, dim, top_k;
+  int parts;                  // CTAs a token
 };
 
 // out[t] = sum over j of weights[t, j] * y[positions[t, j]], in fp32 in the order of j; eight values a thread.
 template <typename T>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const CombineParams p) {
   wait_for_primary();   // the down product's rows
-  const int vectors = p.dim >> 3;
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const long long token = i / vectors;
-  if (token >= p.tokens) return;
-  const int col = static_cast<int>(i - token * vectors) * 8;
+  const unsigned token = blockIdx.x / static_cast<unsigned>(p.parts);   // (the same for the whole CTA)
+  const int col = 8 * static_cast<int>((blockIdx.x - token * p.parts) * kCombineThreads + threadIdx.x);
+  if (col >= p.dim) return;
   const long long pairs = static_cast<long long>(p.tokens) * p.top_k;
   float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
   for (int j = 0; j < p.top_k; ++j) {
-    const long long row = __ldg(p.positions + token * p.top_k + j);
-    const float w = __ldg(p.weights + token * p.top_k + j);
+    const long long row = __ldg(p.positions + static_cast<size_t>(token) * p.top_k + j);
+    const float w = __ldg(p.weights + static_cast<size_t>(token) * p.top_k + j);
     if (row < 0 || row >= pairs) continue;
-    float v[8];
-    unpack16<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + row * p.dim + col), v);
+    const float4* y = reinterpret_cast<const float4*>(p.y + row * p.dim + col);
+    const float4 a = y[0], b = y[1];
+    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int x = 0; x < 8; ++x) sum[x] = fmaf(w, v[x], sum[x]);
   }
-  *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + token * p.dim + col) = pack16<T>(sum);
+  *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + static_cast<size_t>(token) * p.dim + col) = pack16<T>(sum);
 }
 
 template <typename T>
-cudaError_t launch_combine(const CombineParams& p, cudaStream_t stream) {
-  const long long threads = static_cast<long long>(p.tokens) * (p.dim >> 3);
+cudaError_t launch_combine(CombineParams p, cudaStream_t stream) {
+  p.parts = (p.dim / 8 + kCombineThreads - 1) / kCombineThreads;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((threads + kCombineThreads - 1) / kCombineThreads));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.tokens) * static_cast<unsigned>(p.parts));
   cfg.blockDim = dim3(kCombineThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -72,7 +75,7 @@ Plan plan_of(const fmoe_fp8_experts_args& a) {
   pl.xs = take(pairs * blocks_of(a.token_dim) * sizeof(float));
   pl.hq = take(pairs * a.ffn_size);
   pl.hs = take(pairs * blocks_of(a.ffn_size) * sizeof(float));
-  pl.y = take(pairs * a.token_dim * element_bytes(a.data_type));
+  pl.y = take(pairs * a.token_dim * sizeof(float));
   pl.total = at;
   return pl;
 }
@@ -90,6 +93,8 @@ int check_shape(const fmoe_fp8_experts_args* a) {
     return set_error(FMOE_ERR_UNSUPPORTED, "the 8-bit expert layer handles BF16 and FP16 tokens");
   if (static_cast<long long>(a->num_tokens) * a->top_k > 0x7fff0000ll)
     return set_error(FMOE_ERR_UNSUPPORTED, "num_tokens * top_k must fit 32 bits");
+  if (static_cast<long long>(a->num_tokens) * (a->token_dim / (8 * kCombineThreads) + 1) > 0x7fff0000ll)
+    return set_error(FMOE_ERR_UNSUPPORTED, "num_tokens * token_dim is more than a grid holds (32 bits of CTAs)");
   return FMOE_OK;
 }
 
@@ -135,7 +140,7 @@ int fmoe_fp8_experts(const fmoe_fp8_experts_args* a, void* stream) {
                                   ws + pl.hq, reinterpret_cast<float*>(ws + pl.hs), a->offsets, pairs, a->ffn_size,
                                   a->token_dim, a->num_experts, a->act_type, a->device_id};
   const fmoe_fp8_matmul_args down{ws + pl.hq, reinterpret_cast<float*>(ws + pl.hs), a->down, a->down_scale, ws + pl.y, a->offsets,
-                                  pairs, a->token_dim, a->ffn_size, a->num_experts, a->data_type, a->device_id};
+                                  pairs, a->token_dim, a->ffn_size, a->num_experts, FMOE_DT_FP32, a->device_id};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   rc = gated_matmul(&gated, Launch::kCheckOnly, st);   // what any of the steps refuses is refused before the first
   if (rc == FMOE_OK) rc = matmul(&down, Launch::kCheckOnly, st);
@@ -145,7 +150,7 @@ int fmoe_fp8_experts(const fmoe_fp8_experts_args* a, void* stream) {
   if (rc != FMOE_OK) return rc;
   OnDevice on(a->device_id);
   if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));
-  const CombineParams c{ws + pl.y, a->positions, a->weights, a->out, a->num_tokens, a->token_dim, a->top_k};
+  const CombineParams c{reinterpret_cast<float*>(ws + pl.y), a->positions, a->weights, a->out, a->num_tokens, a->token_dim, a->top_k, 0};
   const cudaError_t e = a->data_type == FMOE_DT_BF16 ? launch_combine<__nv_bfloat16>(c, st)
                                                      : launch_combine<__half>(c, st);
   if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("combine launch: ") + cudaGetErrorString(e));

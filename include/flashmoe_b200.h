@@ -364,8 +364,8 @@ typedef struct fmoe_fp8_gated_args {
 int fmoe_fp8_gated_matmul(const fmoe_fp8_gated_args* args, void* stream);
 
 /* The expert layer on 8-bit weights: tokens are quantised into expert order, multiplied with up and
- * up_v, activated and quantised, multiplied with down (rounded to data_type, as the rows that
- * fmoe_forward returns) and summed per token in fp32 in the order of its choices, one rounding. */
+ * up_v, activated and quantised, multiplied with down, and summed per token in the order of its
+ * choices: in fp32 throughout, but for the two quantisations and one rounding at the end. */
 typedef struct fmoe_fp8_experts_args {
   const void* tokens;       /* [num_tokens, token_dim] of data_type; 16-byte aligned */
   const int32_t* offsets;   /* [num_experts + 1], of fmoe_router_select */
