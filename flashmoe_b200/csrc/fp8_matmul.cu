@@ -987,13 +987,17 @@ const DeviceFacts& facts(int device) {
   return all[device];
 }
 
-// Launches a kernel in clusters of `cluster` CTAs.
+// Launches a kernel in clusters of `cluster` CTAs; `registers`: what its warps will share out among themselves.
 template <typename Kernel>
-int launch_kernel(Kernel kernel, std::atomic<unsigned long long>& prepared, size_t smem, int threads, int grid, int cluster,
-                  const CUtensorMap (&maps)[3], const ProductParams& p, int device, cudaStream_t stream) {
+int launch_kernel(Kernel kernel, std::atomic<unsigned long long>& prepared, size_t smem, int threads, int registers, int grid,
+                  int cluster, const CUtensorMap (&maps)[3], const ProductParams& p, int device, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
-  if (!(prepared.load(std::memory_order_acquire) >> device & 1)) {   // once a device: raise the shared-memory limit
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (!(prepared.load(std::memory_order_acquire) >> device & 1)) {   // once a device
+    cudaFuncAttributes made;
+    e = cudaFuncGetAttributes(&made, kernel);
+    if (e == cudaSuccess && made.numRegs * threads < registers)   // (a warp would wait for registers that do not exist)
+      return set_error(FMOE_ERR_UNSUPPORTED, "the 8-bit product was compiled with fewer registers than its warps share out");
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("8-bit product: ") + cudaGetErrorString(e));
     prepared.fetch_or(1ull << device, std::memory_order_release);
   }
@@ -1026,15 +1030,16 @@ int launch_kernel(Kernel kernel, std::atomic<unsigned long long>& prepared, size
 template <typename Out, bool kPair>
 int launch_wide(const ProductParams& p, const CUtensorMap (&maps)[3], int grid, int device, cudaStream_t stream) {
   static std::atomic<unsigned long long> prepared{0};
-  return launch_kernel(product_kernel<Out, kPair>, prepared, Wide<kPair>::smem_bytes(), kThreads, grid, kPair ? 2 : 1, maps, p,
-                       device, stream);
+  constexpr int kRegisters = 32 * (kEpilogueWarp * kLoadRegs + kEpilogueWarps * kEpilogueRegs);
+  return launch_kernel(product_kernel<Out, kPair>, prepared, Wide<kPair>::smem_bytes(), kThreads, kRegisters, grid,
+                       kPair ? 2 : 1, maps, p, device, stream);
 }
 template <typename Out, int kRows>
 int launch_narrow(const ProductParams& p, const CUtensorMap (&maps)[3], int grid, int splits, int device, cudaStream_t stream) {
   using N = Narrow<std::is_same_v<Out, Codes>, kRows>;
   static_assert(N::kSmem <= 227 * 1024, "shared memory of one CTA");
   static std::atomic<unsigned long long> prepared{0};
-  return launch_kernel(product_narrow_kernel<Out, kRows>, prepared, N::kSmem, kNarrowThreads, grid, splits, maps, p, device, stream);
+  return launch_kernel(product_narrow_kernel<Out, kRows>, prepared, N::kSmem, kNarrowThreads, 0, grid, splits, maps, p, device, stream);
 }
 
 // Which kernel a product takes, and its launch shape.
