@@ -85,7 +85,13 @@ struct FastQuantizer {
   }
   __device__ __forceinline__ float scaled(float x) const { return (x * pre) * inv; }
 };
-__device__ __forceinline__ float block_scale(float amax) { return __fdiv_rn(amax, kE4m3Max); }
+// amax / 448 correctly rounded, in the same way; tiny ones, whose quotient loses bits, by a division.
+__device__ __forceinline__ float block_scale(float amax) {
+  if (!(amax >= 0x1p-90f && amax <= 0x1p+120f)) return __fdiv_rn(amax, kE4m3Max);
+  constexpr float r = 1.0f / kE4m3Max;
+  const float y = amax * r;
+  return fmaf(fmaf(-kE4m3Max, y, amax), r, y);
+}
 // Two values to two codes (lo in the low byte), round to nearest even.
 __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
   uint16_t r;

@@ -6,9 +6,6 @@
 namespace fmoe::fp8 {
 namespace {
 
-// From this many blocks on (the GPU full of threads twice over) a thread takes two.
-constexpr long long kTwiceFrom = 2 * 148 * 64 * 4;
-
 struct QuantizeParams {
   const void* x;
   unsigned char* q;
@@ -17,22 +14,14 @@ struct QuantizeParams {
   int copies;
   int rows, cols;
   int row_blocks, col_blocks;
+  unsigned long long per_row;   // rows: 2^64 / col_blocks + 1
 };
 
-// 16 consecutive values as loaded.
-template <typename T>
-struct Raw16 {
-  static constexpr int kPieces = static_cast<int>(sizeof(T));
-  static constexpr int kPer = 16 / sizeof(T);
+// A thread's share of a block, kPieces pieces of 16 bytes: as loaded, their largest value, their codes.
+template <typename T, int kPieces>
+struct Raw {
+  static constexpr int kPer = 16 / sizeof(T);   // values of a piece
   uint4 u[kPieces];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) u[i] = make_uint4(0, 0, 0, 0);
-  }
   // The largest |x|, as bits that order like the value (16-bit types: their own bits, two at a time).
   __device__ __forceinline__ uint32_t amax_bits() const {
     uint32_t m = 0;
@@ -53,62 +42,74 @@ struct Raw16 {
     else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(bits << 16);
     else return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
   }
-  __device__ __forceinline__ uint4 codes(const Quantizer& z) const {
-    float f[16];
+  // four codes to a word
+  __device__ __forceinline__ void codes(const Quantizer& z, uint32_t (&w)[kPieces * kPer / 4]) const {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      float part[kPer];
-      unpack16<T>(u[i], part);
+      float f[kPer];
+      unpack16<T>(u[i], f);
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) f[i * kPer + j] = part[j];
+      for (int j = 0; j < kPer / 4; ++j) {
+        const float2 a = z.scaled(f[4 * j], f[4 * j + 1]), b = z.scaled(f[4 * j + 2], f[4 * j + 3]);
+        w[i * (kPer / 4) + j] = to_e4m3x4(a.x, a.y, b.x, b.y);
+      }
     }
-    uint32_t w[4];
+  }
+};
+template <typename T>
+struct Raw16 : Raw<T, sizeof(T)> {   // 16 consecutive values
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 a = z.scaled(f[4 * i], f[4 * i + 1]), b = z.scaled(f[4 * i + 2], f[4 * i + 3]);
-      w[i] = to_e4m3x4(a.x, a.y, b.x, b.y);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) this->u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) this->u[i] = make_uint4(0, 0, 0, 0);
   }
 };
 
-// Eight threads a block of 128, sixteen values each; kTwice: two blocks a thread, both loaded before either is used.
-template <typename T, bool kTwice>
+// A block of 128 by kLanes threads, whose pieces of 16 bytes alternate, so that a load and a store of theirs lie side by
+// side.  What a block costs besides its values (its place, the reciprocal, the scale) is shared by few lanes: with
+// eight a block, 16 values each, that was half of the instructions.
+template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams p) {
   launch_dependents();   // (of the expert layer: its next kernel)
-  constexpr int kEach = kTwice ? 2 : 1, kBlocks = 32 * kEach;   // blocks of a thread, of a CTA
-  const int sub = threadIdx.x & 7;
-  Raw16<T> raw[kEach];
-  uint32_t row[kEach];
-  int cb[kEach], col[kEach];
-  bool in[kEach];
+  constexpr int kLanes = 4, kPer = 16 / sizeof(T), kPieces = kBlock / kPer / kLanes;
+  const int sub = threadIdx.x & (kLanes - 1);
+  const uint32_t block = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;   // (the host sees to it that it fits)
+  // block / col_blocks: the high half of block * (2^64 / col_blocks + 1) (exact for 32-bit numbers)
+  const uint32_t row = p.col_blocks == 1 ? block : static_cast<uint32_t>(__umul64hi(block, p.per_row));
+  const int cb = static_cast<int>(block - row * p.col_blocks), col = cb * kBlock + sub * kPer;
+  const bool live = row < static_cast<uint32_t>(p.rows);
+  const T* x = static_cast<const T*>(p.x) + static_cast<size_t>(row) * p.cols + col;
+  Raw<T, kPieces> raw;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const uint32_t block = blockIdx.x * kBlocks + 32 * i + (threadIdx.x >> 3);   // (the host sees to it that it fits)
-    row[i] = block / static_cast<uint32_t>(p.col_blocks);
-    cb[i] = static_cast<int>(block - row[i] * p.col_blocks);
-    col[i] = cb[i] * kBlock + sub * 16;
-    in[i] = row[i] < static_cast<uint32_t>(p.rows) && col[i] < p.cols;   // (cols is a multiple of 16)
-    raw[i].zero();
-    if (in[i]) raw[i].load(static_cast<const T*>(p.x) + static_cast<size_t>(row[i]) * p.cols + col[i]);
+  for (int i = 0; i < kPieces; ++i) {
+    raw.u[i] = make_uint4(0, 0, 0, 0);
+    if (live && col + i * kLanes * kPer < p.cols) raw.u[i] = __ldg(reinterpret_cast<const uint4*>(x + i * kLanes * kPer));
   }
+  uint32_t m = raw.amax_bits();
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    uint32_t m = raw[i].amax_bits();
-#pragma unroll
-    for (int d = 1; d < 8; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const float amax = Raw16<T>::amax_value(m);
-    const uint4 codes = raw[i].codes(Quantizer(amax));
-    if (row[i] >= static_cast<uint32_t>(p.rows)) continue;
-    for (int j = 0; j < p.copies; ++j) {
-      long long to = row[i];
-      if (p.positions != nullptr) {
-        to = __ldg(p.positions + static_cast<size_t>(row[i]) * p.copies + j);
-        if (to < 0 || to >= static_cast<long long>(p.rows) * p.copies) continue;
-      }
-      if (in[i]) *reinterpret_cast<uint4*>(p.q + to * p.cols + col[i]) = codes;
-      if (sub == 0) p.scale[to * p.col_blocks + cb[i]] = block_scale(amax);
+  for (int d = 1; d < kLanes; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if (!live) return;
+  const float amax = raw.amax_value(m);
+  uint32_t codes[kPieces * kPer / 4];
+  raw.codes(Quantizer(amax), codes);
+  for (int j = 0; j < p.copies; ++j) {
+    long long to = row;
+    if (p.positions != nullptr) {
+      to = __ldg(p.positions + static_cast<size_t>(row) * p.copies + j);
+      if (to < 0 || to >= static_cast<long long>(p.rows) * p.copies) continue;
     }
+    unsigned char* q = p.q + to * p.cols + col;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      if (col + i * kLanes * kPer < p.cols) {
+        if constexpr (kPer == 8) *reinterpret_cast<uint2*>(q + i * kLanes * kPer) = make_uint2(codes[2 * i], codes[2 * i + 1]);
+        else *reinterpret_cast<uint32_t*>(q + i * kLanes * kPer) = codes[i];
+      }
+    }
+    if (sub == 0) p.scale[to * p.col_blocks + cb] = block_scale(amax);
   }
 }
 
@@ -139,8 +140,11 @@ __global__ void __launch_bounds__(256) quantize_weights_kernel(const QuantizePar
   const Quantizer z(amax);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (row0 + 32 * i < p.rows && col < p.cols)
-      *reinterpret_cast<uint4*>(p.q + base + static_cast<size_t>(row0 + 32 * i) * p.cols) = raw[i].codes(z);
+    if (row0 + 32 * i < p.rows && col < p.cols) {
+      uint32_t w[4];
+      raw[i].codes(z, w);
+      *reinterpret_cast<uint4*>(p.q + base + static_cast<size_t>(row0 + 32 * i) * p.cols) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
   if (threadIdx.x == 0) p.scale[(matrix * p.row_blocks + rb) * p.col_blocks + cb] = block_scale(amax);
 }
@@ -149,8 +153,7 @@ template <typename T>
 cudaError_t launch(const QuantizeParams& p, int block_rows, int matrices, cudaStream_t stream) {
   if (block_rows == 1) {
     const long long blocks = static_cast<long long>(p.rows) * p.col_blocks;
-    if (blocks >= kTwiceFrom) quantize_rows_kernel<T, true><<<static_cast<unsigned>((blocks + 63) / 64), 256, 0, stream>>>(p);
-    else quantize_rows_kernel<T, false><<<static_cast<unsigned>((blocks + 31) / 32), 256, 0, stream>>>(p);
+    quantize_rows_kernel<T><<<static_cast<unsigned>((blocks + 63) / 64), 256, 0, stream>>>(p);
   } else {
     quantize_weights_kernel<T><<<dim3(static_cast<unsigned>(p.row_blocks * p.col_blocks), matrices), 256, 0, stream>>>(p);
   }
@@ -185,9 +188,10 @@ extern "C" int fmoe_fp8_quantize(const fmoe_fp8_quantize_args* a, void* stream) 
   if (misaligned(a->x, 16) || misaligned(a->q, 16)) return set_error(FMOE_ERR_INVALID_ARG, "x and q must be 16-byte aligned");
   if (misaligned(a->scale, 4) || misaligned(a->positions, 4))
     return set_error(FMOE_ERR_INVALID_ARG, "scale and positions must be 4-byte aligned");
-  QuantizeParams p{a->x, static_cast<unsigned char*>(a->q), a->scale, a->positions, a->copies, a->rows, a->cols, 0, 0};
+  QuantizeParams p{a->x, static_cast<unsigned char*>(a->q), a->scale, a->positions, a->copies, a->rows, a->cols, 0, 0, 0};
   p.row_blocks = a->block_rows == 1 ? a->rows : blocks_of(a->rows);
   p.col_blocks = blocks_of(a->cols);
+  p.per_row = ~0ull / p.col_blocks + 1;
   int matrices = a->num_matrices;
   if (a->block_rows == 1) {   // rows of several matrices are just more rows
     if (static_cast<long long>(a->rows) * matrices > 0x7fffffffll)
