@@ -209,10 +209,32 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64
       : "memory");
 }
 // ---- programmatic launches ------------------------------------------------------------------------
-// The next grid may start when every CTA of this one has said so, and waits for this one's
-// results where it needs them.
+// Every kernel here is launched so that it may start while the stream's last kernel runs: it sets up, waits for that
+// kernel to be complete before it touches global memory, and then lets the next one start likewise.  A kernel
+// that waits is complete only after the one before it, so the stream's order holds throughout.  (Inside the expert
+// layer a kernel may read before the wait what was complete before the layer began.)
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Expected, typename... Given>
+cudaError_t launch_behind(void (*kernel)(Expected...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
+                          Given&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  ++g_launches;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 // ---- host side -----------------------------------------------------------------------------------
 constexpr int kMaxDevices = 64;
@@ -233,9 +255,9 @@ struct OnDevice {
   OnDevice& operator=(const OnDevice&) = delete;
 };
 inline bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
-// The products.  kDependent: launched under the tail of the stream's last kernel, which writes A and was itself launched
-// after everything else was complete; kCheckOnly: the arguments are looked at, nothing is launched.
-enum class Launch { kPlain, kDependent, kCheckOnly };
+// The products.  kInLayer: the stream's last kernel writes A, and everything else was complete before it let this one
+// start; kCheckOnly: the arguments are looked at, nothing is launched.
+enum class Launch { kPlain, kInLayer, kCheckOnly };
 int matmul(const fmoe_fp8_matmul_args* a, Launch how, cudaStream_t stream);
 int gated_matmul(const fmoe_fp8_gated_args* a, Launch how, cudaStream_t stream);
 inline int element_bytes(int data_type) { return data_type == FMOE_DT_FP32 ? 4 : 2; }

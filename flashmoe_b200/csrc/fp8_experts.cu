@@ -1,9 +1,8 @@
 // The expert layer on 8-bit weights as a chain of four launches: quantise the tokens into expert
 // order, gated up product (activation and quantisation in its epilogue), down product, weighted sum.
-// Each but the first is launched under the tail of the one before: it sets up, and the few-row products fetch their
-// first weights, before it waits for what that one writes.  The first is an ordinary launch, so whatever the chain
-// reads from outside is complete by then; every CTA of every kernel waits before it ends, so the end of the last one
-// is the end of all.
+// The first waits for whatever the layer reads from outside before it lets the second start; from there on each
+// kernel sets up, and the few-row products fetch their first weights, before they wait for what the one before writes.
+// Every CTA of every kernel waits before it ends, so the end of the last one is the end of all.
 //
 // The down product's rows stay in fp32 until they are summed: in 16 bits they would be half the bytes, a few per cent
 // of a large layer's time, and their rounding would add as much error again as the one at the end.
@@ -49,17 +48,8 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const CombineP
 template <typename T>
 cudaError_t launch_combine(CombineParams p, cudaStream_t stream) {
   p.parts = (p.dim / 8 + kCombineThreads - 1) / kCombineThreads;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.tokens) * static_cast<unsigned>(p.parts));
-  cfg.blockDim = dim3(kCombineThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  ++g_launches;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<T>, p);
+  return launch_behind(combine_kernel<T>, dim3(static_cast<unsigned>(p.tokens) * static_cast<unsigned>(p.parts)), kCombineThreads,
+                       0, 1, stream, p);
 }
 
 // Parts of the workspace, each 256-byte aligned.
@@ -145,8 +135,8 @@ int fmoe_fp8_experts(const fmoe_fp8_experts_args* a, void* stream) {
   rc = gated_matmul(&gated, Launch::kCheckOnly, st);   // what any of the steps refuses is refused before the first
   if (rc == FMOE_OK) rc = matmul(&down, Launch::kCheckOnly, st);
   if (rc == FMOE_OK) rc = fmoe_fp8_quantize(&quantize, stream);
-  if (rc == FMOE_OK) rc = gated_matmul(&gated, Launch::kDependent, st);
-  if (rc == FMOE_OK) rc = matmul(&down, Launch::kDependent, st);
+  if (rc == FMOE_OK) rc = gated_matmul(&gated, Launch::kInLayer, st);
+  if (rc == FMOE_OK) rc = matmul(&down, Launch::kInLayer, st);
   if (rc != FMOE_OK) return rc;
   OnDevice on(a->device_id);
   if (on.err != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(on.err));

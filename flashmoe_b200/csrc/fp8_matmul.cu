@@ -51,7 +51,7 @@ struct ProductParams {
   float* out_scale;            // gated form
   int act, has_v;              // gated form
   int wide;                    // output rows may be stored 32 bytes at a time
-  int dependent;               // launched under the tail of the kernel that writes A (weights and offsets are older)
+  int in_layer;                // weights and offsets may be read before the wait for the kernel that writes A
   long long spin_limit;
 };
 
@@ -297,13 +297,14 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       tmem_relinquish();
     }
   }
+  if (!p.in_layer) wait_for_primary();
   fill_table(sh.table, p, kTileM);
   if constexpr (kPair) cluster_sync_all();   // both CTAs' barriers exist before either is signalled from the other
   tc_fence_after_sync();
   const uint32_t tmem = sh.tmem_base;
   const bool second = !kGated || p.has_v != 0;   // whether the second 128 weight rows exist
   launch_dependents();
-  if (p.dependent) wait_for_primary();
+  if (p.in_layer) wait_for_primary();
 
   if (warp < kEpilogueWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
@@ -667,13 +668,14 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     tmem_alloc(&sh.tmem_base, N::kTmemColumns);
     tmem_relinquish();
   }
+  if (!p.in_layer) wait_for_primary();
   fill_table(sh.table, p, kRows);
   if (splits > 1) cluster_sync_all();   // the others' barriers exist before any is signalled
   tc_fence_after_sync();
   const uint32_t tmem = sh.tmem_base;
   const bool second = kGated && p.has_v != 0;
   launch_dependents();
-  if (p.dependent && warp != 0) wait_for_primary();
+  if (p.in_layer && warp != 0) wait_for_primary();
 
   if (warp == 0) {
     const uint32_t bytes = N::kRowBytes + (second ? 2 : 1) * kBoxBytes;
@@ -681,7 +683,7 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     Tile t;
     bool ok = true;
     int early = 0;   // blocks whose weights are on their way before the rows exist
-    if (p.dependent) {
+    if (p.in_layer) {
       if (find_tile(sh.table, p, first_tile, kRows, kBlock, t)) {
         early = min(kStages, kb1 - kb0);
         if (elect_one()) {
@@ -1001,28 +1003,7 @@ int launch_kernel(Kernel kernel, std::atomic<unsigned long long>& prepared, size
     if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("8-bit product: ") + cudaGetErrorString(e));
     prepared.fetch_or(1ull << device, std::memory_order_release);
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (cluster > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = cluster;
-    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (p.dependent) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  e = cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], p);
-  ++g_launches;
+  e = launch_behind(kernel, dim3(grid), threads, smem, cluster, stream, maps[0], maps[1], maps[2], p);
   if (e != cudaSuccess) return set_error(FMOE_ERR_CUDA, std::string("8-bit product launch: ") + cudaGetErrorString(e));
   return FMOE_OK;
 }
@@ -1166,7 +1147,7 @@ int matmul(const fmoe_fp8_matmul_args* a, Launch how, cudaStream_t st) {
   p.w_scale[0] = a->w_scale;
   p.out = a->out;
   p.wide = !misaligned(a->out, 32) && (static_cast<size_t>(a->n) * eb) % 32 == 0;
-  p.dependent = how == Launch::kDependent;
+  p.in_layer = how == Launch::kInLayer;
   if (a->data_type == FMOE_DT_BF16) return launch_product<__nv_bfloat16>(p, a->a, a->w, a->w, a->device_id, st);
   if (a->data_type == FMOE_DT_FP16) return launch_product<__half>(p, a->a, a->w, a->w, a->device_id, st);
   return launch_product<float>(p, a->a, a->w, a->w, a->device_id, st);
@@ -1197,7 +1178,7 @@ int gated_matmul(const fmoe_fp8_gated_args* a, Launch how, cudaStream_t st) {
   p.out_scale = a->scale;
   p.act = a->act_type;
   p.has_v = a->up_v != nullptr;
-  p.dependent = how == Launch::kDependent;
+  p.in_layer = how == Launch::kInLayer;
   return launch_product<Codes>(p, a->a, a->up, a->up_v != nullptr ? a->up_v : a->up, a->device_id, st);
 }
 

@@ -73,7 +73,8 @@ struct Raw16 : Raw<T, sizeof(T)> {   // 16 consecutive values
 // eight a block, 16 values each, that was half of the instructions.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams p) {
-  launch_dependents();   // (of the expert layer: its next kernel)
+  wait_for_primary();
+  launch_dependents();
   constexpr int kLanes = 4, kPer = 16 / sizeof(T), kPieces = kBlock / kPer / kLanes;
   const int sub = threadIdx.x & (kLanes - 1);
   const uint32_t block = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;   // (the host sees to it that it fits)
@@ -116,6 +117,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams
 // One CTA a block of 128 x 128: a pass takes 32 rows, eight threads each; four passes stay in registers.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_weights_kernel(const QuantizeParams p) {
+  wait_for_primary();
+  launch_dependents();
   __shared__ uint32_t s_max[8];
   const long long matrix = blockIdx.y;
   const int rb = blockIdx.x / p.col_blocks, cb = blockIdx.x - rb * p.col_blocks;
@@ -153,12 +156,10 @@ template <typename T>
 cudaError_t launch(const QuantizeParams& p, int block_rows, int matrices, cudaStream_t stream) {
   if (block_rows == 1) {
     const long long blocks = static_cast<long long>(p.rows) * p.col_blocks;
-    quantize_rows_kernel<T><<<static_cast<unsigned>((blocks + 63) / 64), 256, 0, stream>>>(p);
-  } else {
-    quantize_weights_kernel<T><<<dim3(static_cast<unsigned>(p.row_blocks * p.col_blocks), matrices), 256, 0, stream>>>(p);
+    return launch_behind(quantize_rows_kernel<T>, dim3(static_cast<unsigned>((blocks + 63) / 64)), 256, 0, 1, stream, p);
   }
-  ++g_launches;
-  return cudaGetLastError();
+  return launch_behind(quantize_weights_kernel<T>, dim3(static_cast<unsigned>(p.row_blocks * p.col_blocks), matrices), 256, 0,
+                       1, stream, p);
 }
 
 }  // namespace

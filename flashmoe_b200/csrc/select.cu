@@ -421,6 +421,7 @@ __host__ __device__ __forceinline__ size_t row_doubles(int E, int groups) { retu
 template <int V>
 __global__ void __launch_bounds__(256) select_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ __align__(16) unsigned char s_raw[];
+  fp8::wait_for_primary();
   fp8::launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.x * 8 + warp;
@@ -466,7 +467,7 @@ __device__ __forceinline__ unsigned lanes_alike(int id, int bits) {
 // One CTA per expert that scans all pairs for itself needs no steps but reads the pairs once per expert: 65536 pairs
 // of 128 experts took 18 us.
 template <int kCtas>
-__device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bool dependent) {
+__device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bool behind) {
   __shared__ int s_sum[kOrderWarps];
   const int E = p.E, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = kCtas > 1 ? blockIdx.x : 0;     // (the grid is one cluster)
@@ -474,7 +475,10 @@ __device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bo
   int* total = hist + kOrderWarps * E;            // [E]: this CTA's pairs
   for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) hist[i] = 0;
   __syncthreads();
-  if (dependent) fp8::wait_for_primary();              // the ids are another grid's
+  if (behind) {                                   // the ids are another grid's
+    fp8::wait_for_primary();
+    fp8::launch_dependents();
+  }
   const long long pairs = static_cast<long long>(p.S) * p.k;
   constexpr long long kWorkers = static_cast<long long>(kCtas) * kOrderWarps;
   const long long share = ((pairs + kWorkers - 1) / kWorkers + 31) & ~31ll;
@@ -578,13 +582,15 @@ __device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bo
 template <int kCtas>
 __global__ void __launch_bounds__(kOrderThreads) order_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ __align__(16) unsigned char s_raw[];
-  order_pairs<kCtas>(p, reinterpret_cast<int*>(s_raw), p.S > 0);
+  order_pairs<kCtas>(p, reinterpret_cast<int*>(s_raw), true);
 }
 
 // Few tokens: one CTA chooses and orders.
 template <int V>
 __global__ void __launch_bounds__(kOrderThreads) select_few_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ __align__(16) unsigned char s_raw[];
+  fp8::wait_for_primary();
+  fp8::launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int token = warp; token < p.S; token += kOrderWarps)
     select_token<V>(p, token, lane, reinterpret_cast<double*>(s_raw) + warp * row_doubles(p.E, p.groups));
@@ -593,34 +599,12 @@ __global__ void __launch_bounds__(kOrderThreads) select_few_kernel(const __grid_
 }
 
 template <typename Kernel>
-cudaError_t launch(Kernel kernel, const SelectParams& p, int grid, int threads, size_t smem, int cluster, bool dependent,
-                   cudaStream_t stream) {
+cudaError_t launch(Kernel kernel, const SelectParams& p, int grid, int threads, size_t smem, int cluster, cudaStream_t stream) {
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (cluster > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = cluster;
-    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-    ++n;
-  }
-  if (dependent) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  ++g_launches;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return fp8::launch_behind(kernel, dim3(grid), threads, smem, cluster, stream, p);
 }
 
 // Up to this many tokens one CTA does it all, in two rounds of its 32 warps.
@@ -633,19 +617,19 @@ cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
   if constexpr (V <= 8) {   // (the registers of 32 warps)
     if (p.S <= kFewTokens) {
       const size_t rows = kOrderWarps * group_row;
-      return launch(select_few_kernel<V>, p, 1, kOrderThreads, rows > order ? rows : order, 1, false, stream);
+      return launch(select_few_kernel<V>, p, 1, kOrderThreads, rows > order ? rows : order, 1, stream);
     }
   }
   if (p.S > 0) {
-    const cudaError_t e = launch(select_kernel<V>, p, (p.S + 7) / 8, 256, 8 * group_row, 1, false, stream);
+    const cudaError_t e = launch(select_kernel<V>, p, (p.S + 7) / 8, 256, 8 * group_row, 1, stream);
     if (e != cudaSuccess) return e;
   }
   // (both kernels, 65536 pairs of 128 experts: 18.5 us by 8 CTAs, 16.4 by 16; 16384 pairs of 256 experts: 15.1 and 14.4)
   const long long pairs = static_cast<long long>(p.S) * p.k;
-  if (pairs <= kOrderThreads) return launch(order_kernel<1>, p, 1, kOrderThreads, order, 1, p.S > 0, stream);
+  if (pairs <= kOrderThreads) return launch(order_kernel<1>, p, 1, kOrderThreads, order, 1, stream);
   const cudaError_t e = cudaFuncSetAttribute(order_kernel<16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
-  return launch(order_kernel<16>, p, 16, kOrderThreads, order, 16, p.S > 0, stream);
+  return launch(order_kernel<16>, p, 16, kOrderThreads, order, 16, stream);
 }
 
 int check(const fmoe_select_args* a) {
