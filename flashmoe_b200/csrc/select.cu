@@ -169,10 +169,9 @@ __device__ __forceinline__ uint32_t alive_bits(int E, int groups, uint32_t kept,
   return alive;
 }
 
-// The row decided in 64 bits; lane j < k leaves with the j-th choice.
+// What is compared, in 64 bits.
 template <int V>
-__device__ __noinline__ int choose_exactly(const SelectParams& p, size_t row, int lane, double* shared_row) {
-  double c[V];
+__device__ __forceinline__ void exact_scores(const SelectParams& p, size_t row, int lane, double (&c)[V]) {
   double top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -196,22 +195,29 @@ __device__ __noinline__ int choose_exactly(const SelectParams& p, size_t row, in
     if (p.score == FMOE_SCORE_SOFTMAX && sum > 0.0) c[i] /= sum;
     if (p.bias != nullptr && e < p.E) c[i] += static_cast<double>(sane(__ldg(p.bias + e)));
   }
-  uint32_t kept = kAll;
-  if (p.groups > 1) {
-    const float per = static_cast<float>(p.groups) / static_cast<float>(p.E);
-    __syncwarp();
+}
+
+// The groups that stay, decided in 64 bits.
+template <int V>
+__device__ __noinline__ uint32_t exact_groups(const SelectParams& p, size_t row, int lane, double* shared_row) {
+  double c[V];
+  exact_scores<V>(p, row, lane, c);
+  const float per = static_cast<float>(p.groups) / static_cast<float>(p.E);
+  __syncwarp();
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (lane + 32 * i < p.E) shared_row[lane + 32 * i + group_of(lane + 32 * i, per)] = c[i];
-    __syncwarp();
-    double worst, best;
-    kept = kept_groups<double>(group_score<double>(shared_row, p.E, p.groups, p.group_max, lane), p.groups, p.top_groups,
-                               lane, worst, best);
-  }
-  if (p.bias == nullptr) {   // the groups were the question
-#pragma unroll
-    for (int i = 0; i < V; ++i) c[i] = lane + 32 * i < p.E ? static_cast<double>(logit_at(p, row + lane + 32 * i)) : 0.0;
-  }
+  for (int i = 0; i < V; ++i)
+    if (lane + 32 * i < p.E) shared_row[lane + 32 * i + group_of(lane + 32 * i, per)] = c[i];
+  __syncwarp();
+  double worst, best;
+  return kept_groups<double>(group_score<double>(shared_row, p.E, p.groups, p.group_max, lane), p.groups, p.top_groups, lane,
+                             worst, best);
+}
+
+// The choice among the experts of the groups that stay, decided in 64 bits; lane j < k leaves with the j-th.
+template <int V>
+__device__ __noinline__ int choose_exactly(const SelectParams& p, size_t row, int lane, uint32_t kept) {
+  double c[V];
+  exact_scores<V>(p, row, lane, c);
   uint32_t alive = alive_bits<V>(p.E, p.groups, kept, lane);
   int mine = 0;
   for (int r = 0; r < p.k; ++r) {
@@ -260,11 +266,11 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
     }
     if (softmax) sum = warp_sum<float>(part);
   }
-  // how far a computed score may be from the true one: sigmoid takes an exp of 1 ulp and two roundings;
-  // softmax also the rounding of l - max (at most 2^-25 of the largest score: x exp(-x) < 1/2) and a sum of
-  // up to 37 additions in a row, all relative to the score, which is at most exp(0) / sum
-  const float error = softmax ? 0x1p-18f / (sum > 0.0f ? sum : 1.0f) : 0x1p-21f;
-  bool unsure = false;
+  // How far a computed score may be from the true one.  Sigmoid: an exp of 1 ulp below 1 (2^-24), the sum (2^-24) and a
+  // quotient of 2 ulp, of a value below 1: 3/2 2^-22.  Softmax: also the rounding of l - max (at most 2^-25 of the
+  // largest score: x exp(-x) < 1/2) and a sum of up to 37 additions in a row, all relative to the score, which is at
+  // most exp(0) / sum.
+  const float error = softmax ? 0x1p-18f / (sum > 0.0f ? sum : 1.0f) : 0x1.8p-22f;
   uint32_t kept = kAll;
   if (by_score) {
 #pragma unroll
@@ -284,8 +290,12 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
       float worst, best;
       kept = kept_groups<float>(group_score<float>(shared, p.E, p.groups, p.group_max, lane), p.groups, p.top_groups, lane,
                                 worst, best);
-      if (p.top_groups < p.groups)
-        unsure = worst - best <= 4.0f * error + 0x1p-21f * (fabsf(worst) + fabsf(best));
+      // a group's sum: two scores, each rounded when its bias was added, and a rounding of its own, none of them over
+      // 2^-24 of twice the largest |c|
+      float size = 0.0f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) size = fmaxf(size, c[i] == -INFINITY ? 0.0f : fabsf(c[i]));
+      if (worst - best <= 4.0f * error + 0x1p-21f * warp_max<float>(size)) kept = exact_groups<V>(p, row, lane, shared_row);
     }
   }
   const bool by_logit = p.bias == nullptr;
@@ -331,7 +341,7 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
   int mine = 0, found = 0;
   uint32_t mine_key = 0;
   float last = 0.0f;
-  bool close = false;
+  bool close = false, unsure = false;   // some are too close; more than a warp can hold
   for (;; ++found) {
     if (by_logit && found == p.k) break;
     const uint32_t key = __reduce_max_sync(kAll, head);
@@ -367,7 +377,7 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
     }
   }
   if (unsure) {                                  // (the same for the whole warp, as everything that follows)
-    mine = choose_exactly<V>(p, row, lane, shared_row);
+    mine = choose_exactly<V>(p, row, lane, kept);
   } else if (close) {
     // the candidates' scores again, in 64 bits, one a lane; each candidate's place is the number that come before it
     double sum64 = 1.0;
@@ -402,7 +412,7 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
     mine = sorted;
   }
   float l = -INFINITY;
-  if (lane < p.k) l = by_logit && !unsure ? key_value(mine_key) : logit_at(p, row + mine);
+  if (lane < p.k) l = by_logit ? key_value(mine_key) : logit_at(p, row + mine);
   // (shares among the chosen do not depend on the largest of all, which may be far above theirs)
   float s = raw_score<float>(l, p.renormalize ? (by_logit ? __shfl_sync(kAll, l, 0) : warp_max<float>(l)) : top, p.score);
   if (softmax && !p.renormalize && sum > 0.0f) s = s / sum;

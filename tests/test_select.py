@@ -193,6 +193,18 @@ def test_scores_that_fp32_cannot_tell_apart(score):
 
 
 @gpu
+def test_groups_whose_large_scores_cancel():
+    """Two experts a group with biases of +-100: what their sums differ by, steps of 2^-17, is what fp32 loses when the
+    scores are added to the biases (half a step of 2^-17 each)."""
+    g = torch.Generator().manual_seed(3)
+    bias = torch.empty(32, 2)
+    bias[:, 0] = 100.0 + torch.randint(0, 64, (32,), generator=g) * 2.0 ** -17
+    bias[:, 1] = -bias[:, 0] + torch.randperm(32, generator=g) * 2.0 ** -17
+    run(normal(64, 64, seed=8, std=1e-4), 4, score="sigmoid", bias=bias.view(-1), groups=32, top_groups=5)
+    run(torch.zeros(3, 64), 2, score="sigmoid", bias=bias.view(-1), groups=32, top_groups=1)
+
+
+@gpu
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("with_bias", [False, True])
 @pytest.mark.parametrize("groups,top_groups", [(1, 1), (4, 2)])
