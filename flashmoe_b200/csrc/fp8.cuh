@@ -216,6 +216,11 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// What another kernel wrote.  A plain load: __ldg promises that the memory never changes while the kernel runs, and could be
+// moved in front of the wait.
+template <typename T>
+__device__ __forceinline__ T fetched(const T* p) { return *p; }
+
 template <typename... Expected, typename... Given>
 cudaError_t launch_behind(void (*kernel)(Expected...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
                           Given&&... args) {

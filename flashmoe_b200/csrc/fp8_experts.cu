@@ -33,8 +33,8 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const CombineP
   float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
   for (int j = 0; j < p.top_k; ++j) {
-    const long long row = __ldg(p.positions + static_cast<size_t>(token) * p.top_k + j);
-    const float w = __ldg(p.weights + static_cast<size_t>(token) * p.top_k + j);
+    const long long row = fetched(p.positions + static_cast<size_t>(token) * p.top_k + j);
+    const float w = fetched(p.weights + static_cast<size_t>(token) * p.top_k + j);
     if (row < 0 || row >= pairs) continue;
     const float4* y = reinterpret_cast<const float4*>(p.y + row * p.dim + col);
     const float4 a = y[0], b = y[1];

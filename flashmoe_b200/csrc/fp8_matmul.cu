@@ -74,8 +74,8 @@ __device__ __forceinline__ void expert_rows(const ProductParams& p, int e, int& 
   begin = 0;
   end = p.m;
   if (p.offsets != nullptr) {
-    begin = min(max(__ldg(p.offsets + e), 0), p.m);
-    end = min(max(__ldg(p.offsets + e + 1), begin), p.m);
+    begin = min(max(fetched(p.offsets + e), 0), p.m);
+    end = min(max(fetched(p.offsets + e + 1), begin), p.m);
   }
 }
 
@@ -406,7 +406,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   #pragma unroll
           for (int x = 0; x < 4; ++x)
   #pragma unroll
-            for (int j = 0; j < 4; ++j) to[x][j] = src[j] != nullptr && kb + x < p.kblocks ? __ldg(src[j] + kb + x) : 0.0f;
+            for (int j = 0; j < 4; ++j) to[x][j] = src[j] != nullptr && kb + x < p.kblocks ? fetched(src[j] + kb + x) : 0.0f;
         };
         fetch(0, next);
         for (int kb0 = 0; ok && kb0 < p.kblocks; kb0 += 4) {
@@ -781,10 +781,10 @@ product_narrow_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
           for (int j = 0; j < kLaneRows; ++j) {
             const int row = t.row0 + lane + 32 * j;
             a_next[j][x] = in && lane + 32 * j < kRows && row < t.row_end
-                               ? __ldg(p.a_scale + static_cast<size_t>(row) * p.kblocks + kb + x) : 0.0f;
+                               ? fetched(p.a_scale + static_cast<size_t>(row) * p.kblocks + kb + x) : 0.0f;
           }
 #pragma unroll
-          for (int h = 0; h < N::kWeights; ++h) w_next[h][x] = in ? __ldg(w[h] + kb + x) : 0.0f;
+          for (int h = 0; h < N::kWeights; ++h) w_next[h][x] = in ? fetched(w[h] + kb + x) : 0.0f;
         }
       };
       fetch(kb0);

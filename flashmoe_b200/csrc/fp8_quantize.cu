@@ -61,7 +61,7 @@ template <typename T>
 struct Raw16 : Raw<T, sizeof(T)> {   // 16 consecutive values
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) this->u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) this->u[i] = fetched(reinterpret_cast<const uint4*>(p) + i);
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
     raw.u[i] = make_uint4(0, 0, 0, 0);
-    if (live && col + i * kLanes * kPer < p.cols) raw.u[i] = __ldg(reinterpret_cast<const uint4*>(x + i * kLanes * kPer));
+    if (live && col + i * kLanes * kPer < p.cols) raw.u[i] = fetched(reinterpret_cast<const uint4*>(x + i * kLanes * kPer));
   }
   uint32_t m = raw.amax_bits();
 #pragma unroll
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams
   for (int j = 0; j < p.copies; ++j) {
     long long to = row;
     if (p.positions != nullptr) {
-      to = __ldg(p.positions + static_cast<size_t>(row) * p.copies + j);
+      to = fetched(p.positions + static_cast<size_t>(row) * p.copies + j);
       if (to < 0 || to >= static_cast<long long>(p.rows) * p.copies) continue;
     }
     unsigned char* q = p.q + to * p.cols + col;

@@ -47,9 +47,9 @@ __device__ __forceinline__ float sane(float x) { return x == x ? fminf(x, FLT_MA
 
 __device__ __forceinline__ float logit_at(const SelectParams& p, size_t i) {
   float x;
-  if (p.dtype == FMOE_DT_FP32) x = __ldg(static_cast<const float*>(p.logits) + i);
-  else if (p.dtype == FMOE_DT_BF16) x = __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.logits) + i));
-  else x = __half2float(__ldg(static_cast<const __half*>(p.logits) + i));
+  if (p.dtype == FMOE_DT_FP32) x = fp8::fetched(static_cast<const float*>(p.logits) + i);
+  else if (p.dtype == FMOE_DT_BF16) x = __bfloat162float(fp8::fetched(static_cast<const __nv_bfloat16*>(p.logits) + i));
+  else x = __half2float(fp8::fetched(static_cast<const __half*>(p.logits) + i));
   return sane(x);
 }
 
@@ -59,7 +59,7 @@ template <int V>
 __device__ __forceinline__ void load_row(const SelectParams& p, size_t row, int lane, float (&v)[V]) {
   auto load = [&](const auto* from) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = lane + 32 * i < p.E ? fp8::to_float(__ldg(from + row + lane + 32 * i)) : -INFINITY;
+    for (int i = 0; i < V; ++i) v[i] = lane + 32 * i < p.E ? fp8::to_float(fp8::fetched(from + row + lane + 32 * i)) : -INFINITY;
   };
   if (p.dtype == FMOE_DT_FP32) load(static_cast<const float*>(p.logits));
   else if (p.dtype == FMOE_DT_BF16) load(static_cast<const __nv_bfloat16*>(p.logits));
@@ -197,7 +197,7 @@ __device__ __forceinline__ void exact_scores(const SelectParams& p, size_t row, 
   for (int i = 0; i < V; ++i) {
     const int e = lane + 32 * i;
     if (p.score == FMOE_SCORE_SOFTMAX && sum > 0.0) c[i] /= sum;
-    if (p.bias != nullptr && e < p.E) c[i] += static_cast<double>(sane(__ldg(p.bias + e)));
+    if (p.bias != nullptr && e < p.E) c[i] += static_cast<double>(sane(fp8::fetched(p.bias + e)));
   }
 }
 
@@ -250,7 +250,7 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
   float v[V], bias[V];
   if (p.bias != nullptr) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) bias[i] = lane + 32 * i < p.E ? __ldg(p.bias + lane + 32 * i) : 0.0f;
+    for (int i = 0; i < V; ++i) bias[i] = lane + 32 * i < p.E ? fp8::fetched(p.bias + lane + 32 * i) : 0.0f;
   }
   load_row<V>(p, row, lane, v);
   float top = -INFINITY;
@@ -398,7 +398,7 @@ __device__ __forceinline__ void select_token(const SelectParams& p, int token, i
       if (l != -INFINITY) {
         exact = raw_score<double>(l, static_cast<double>(top), p.score);
         if (softmax) exact /= sum64;
-        exact += static_cast<double>(sane(__ldg(p.bias + mine)));
+        exact += static_cast<double>(sane(fp8::fetched(p.bias + mine)));
       }
     }
     int place = 0;

@@ -540,6 +540,33 @@ def test_two_graphs_and_eager_calls_of_one_layer():
         layer.check()
 
 
+FIRST_CALL = """
+import sys, torch
+sys.path[:0] = [{root!r}, {tests!r}]
+import test_fp8 as T
+side = torch.cuda.Stream()
+layer = T.Layer(24, 256, 272, 8, 2, stream_ptr=side.cuda_stream)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    layer.step()
+graph.replay()
+torch.cuda.synchronize()
+layer.check()
+"""
+
+
+@gpu
+def test_the_first_call_of_a_process_can_be_a_captured_one():
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=os.path.dirname(here), tests=here)], capture_output=True,
+                          text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
 @gpu
 def test_large_layer_on_every_form():
     """4096 tokens on 4 experts (pairs) and 64 experts (128 rows)."""
