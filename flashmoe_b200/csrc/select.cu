@@ -487,6 +487,8 @@ __device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bo
   const int cta = kCtas > 1 ? blockIdx.x : 0;     // (the grid is one cluster)
   // hist [warps][E]: counts, then places already handed out
   int* total = hist + kOrderWarps * E;            // [E]: this CTA's pairs
+  int* start = total + E;                         // [E]: the expert's first row
+  int* base = start + E;                          // [E]: its pairs in the CTAs before this one
   for (int i = threadIdx.x; i < kOrderWarps * E; i += kOrderThreads) hist[i] = 0;
   __syncthreads();
   if (behind) {                                   // the ids are another grid's
@@ -556,27 +558,23 @@ __device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bo
   __syncthreads();
   int before = lane < warp ? s_sum[lane] : 0;
   before = __reduce_add_sync(kAll, before);
-  const int start = before + sum - all;
-  if constexpr (kCtas > 1) ptx::cluster_sync_all();   // every total has been read
   if (e < E) {
-    total[e] = start;                             // from here on: the expert's first row
-    if (lower != 0) {
-#pragma unroll
-      for (int w = 0; w < kOrderWarps; ++w) hist[w * E + e] += lower;
-    }
+    const int row = before + sum - all;
+    start[e] = row;
+    base[e] = lower;
     if (cta == 0) {
       p.counts[e] = all;
       if (p.offsets != nullptr) {
-        p.offsets[e] = start;
-        if (e == E - 1) p.offsets[E] = start + all;
+        p.offsets[e] = row;
+        if (e == E - 1) p.offsets[E] = row + all;
       }
     }
   }
   __syncthreads();
-  if (p.positions == nullptr && p.table == nullptr) return;
   const bool once = n <= 32 * kAhead;             // the ids are still in registers
   const int id_bits = 32 - __clz(E - 1);          // (E = 1: no bits)
-  for (int i0 = 0; i0 < n; i0 += 32 * kAhead) {
+  const bool placed = p.positions != nullptr || p.table != nullptr;
+  for (int i0 = 0; placed && i0 < n; i0 += 32 * kAhead) {
     if (!once) load(i0);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
@@ -584,13 +582,14 @@ __device__ __forceinline__ void order_pairs(const SelectParams& p, int* hist, bo
       const int id = ahead[j];
       const unsigned same = lanes_alike(id, id_bits);
       const int rank = __popc(same & ((1u << lane) - 1));
-      const int slot = id >= 0 ? mine[id] + rank : 0;
+      const int slot = id >= 0 ? base[id] + mine[id] + rank : 0;
       __syncwarp();
       if (id >= 0 && rank == 0) mine[id] += __popc(same);
       __syncwarp();
-      if (id >= 0) place_pair(p, first + i0 + 32 * j + lane, id, slot, total[id]);
+      if (id >= 0) place_pair(p, first + i0 + 32 * j + lane, id, slot, start[id]);
     }
   }
+  if constexpr (kCtas > 1) ptx::cluster_sync_all();   // no CTA leaves while another reads its totals
 }
 
 template <int kCtas>
@@ -628,7 +627,7 @@ constexpr int kFewTokens = 64;
 template <int V>
 cudaError_t launch_select(const SelectParams& p, cudaStream_t stream) {
   const size_t group_row = row_doubles(p.E, p.groups) * sizeof(double);
-  const size_t order = static_cast<size_t>(kOrderWarps + 1) * p.E * sizeof(int);
+  const size_t order = static_cast<size_t>(kOrderWarps + 3) * p.E * sizeof(int);
   if constexpr (V <= 8) {   // (the registers of 32 warps)
     if (p.S <= kFewTokens) {
       const size_t rows = kOrderWarps * group_row;
