@@ -16,7 +16,7 @@
 // let the MMAs of one block run while the other block's sums are read.  The same kernel works 128 x 256 tiles by
 // one CTA, for products too small, or experts with too few rows, to fill 256 x 256.
 //
-// Measured: 8192^3 593 us (1855 TFLOP/s), 4096 x 14336 x 4096 268 us (1790).  A block of k takes a pair about 1050
+// Measured: 8192^3 575 to 593 us (1855 to 1910 TFLOP/s), 4096 x 14336 x 4096 266 us (1810).  A block of k takes a pair about 1050
 // cycles: 512 of MMA, 440 to read and multiply-add 256 columns, 600 for the accumulator to change hands twice, over
 // two accumulators.  The MMAs alone would run at 3300.
 #include <atomic>
@@ -578,7 +578,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 // cluster share a tile: each takes a run of the blocks of k, leaves its sums in its shared memory, and adds
 // up, in rank order, the sums of all for its share of the rows.
 //
-// Measured: one row of 8192 x 5120 13 us (42 MB of weights, 6.4 us at the copy rate; the rest is set-up, the first
+// Measured: one row of 8192 x 5120 12.7 us (42 MB of weights, 6.4 us at the copy rate; the rest is set-up, the first
 // load and the cluster's sum), 16 rows of 128 experts of 2048 x 768, up and down, 61 us (389 MB, 59 us).
 
 constexpr int kNarrowThreads = 384;   // TMA, MMA, scale warp, one idle; eight epilogue warps

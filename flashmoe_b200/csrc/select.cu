@@ -9,7 +9,7 @@
 // in 64 bits.  Without a bias the scores are never compared at all: softmax and sigmoid keep the
 // order of the logits, so the logits, which are exact, are (inside a group too).
 //
-// Measured: 8192 tokens of 128 experts 14.4 us, 2048 of 256 experts in 8 groups 13.0 us, one token 4.3 us.  Reading the
+// Measured: 8192 tokens of 128 experts 14.3 us, 2048 of 256 experts in 8 groups 12.6 us, one token 4.2 us.  Reading the
 // logits takes 0.8 us of the first; the rest is instructions (59 % of issue slots) and, in the ordering, a chain of
 // steps that wait for one another.
 #include <cuda_bf16.h>
